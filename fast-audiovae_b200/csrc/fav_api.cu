@@ -22,8 +22,10 @@ static_assert(FAV_SLOT_FLOATS == fav::kSlotFloats, "slot size");
 static_assert(FAV_SLOT_STRIDE_FLOATS == fav::kSlotStride, "slot stride");
 
 namespace {
-
 thread_local char g_error[512] = {0};
+}
+
+namespace fav {
 
 int32_t fail(int32_t status, const char* fmt, ...) {
   va_list ap;
@@ -36,6 +38,15 @@ int32_t fail(int32_t status, const char* fmt, ...) {
 int32_t cuda_fail(cudaError_t e, const char* what) {
   return fail(FAV_DEVICE_ERROR, "%s: %s", what, cudaGetErrorString(e));
 }
+
+void clear_error() { g_error[0] = 0; }
+
+}  // namespace fav
+
+namespace {
+
+using fav::cuda_fail;
+using fav::fail;
 
 // cuTensorMapEncodeTiled from the driver, looked up once through the runtime.
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

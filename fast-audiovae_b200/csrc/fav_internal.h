@@ -7,6 +7,13 @@
 
 namespace fav {
 
+// The thread's last-error string behind fav_last_error (fav_api.cu): record a
+// message and return ``status``; clear it at the start of a call.
+int32_t fail(int32_t status, const char* fmt, ...);
+int32_t cuda_fail(cudaError_t e, const char* what);
+void clear_error();
+
+
 constexpr int kTileM = 128;       // GEMM rows (time steps) per CTA tile
 constexpr int kKBlock = 64;       // K elements (channels) per pipeline stage
 constexpr int kLatentChannels = 64;

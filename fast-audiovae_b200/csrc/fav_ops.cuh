@@ -1,0 +1,145 @@
+// Shared by the stream operators (fav_conv.cu, fav_scan.cu, fav_norm.cu,
+// fav_int4.cu): element types, vector loads and stores, and how packed rows
+// belong to sequences and sequences to state slots.
+#pragma once
+#include "../../include/fast_audiovae_cuda.h"
+#include "fav_device.cuh"
+#include "fav_internal.h"
+
+namespace fav {
+
+// Codes an operator records in the caller's status word (first error wins).
+constexpr uint32_t kDevBadOffsets = 0x201;  // offsets decrease or leave the rows
+constexpr uint32_t kDevBadSlot = 0x202;     // a slot code names no slot of the pool
+
+// ------------------------------------------------------------ element types
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+
+// The one rounding of a result to its stored type (nearest, ties to even).
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// V consecutive elements, moved by one access of V * sizeof(T) bytes.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+  *reinterpret_cast<Pack<T, V>*>(p) = v;
+}
+
+__device__ __forceinline__ float ex2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// v / (1 + e^-v); at -inf the quotient of -inf by +inf is replaced by its limit.
+__device__ __forceinline__ float silu(float v) {
+  const float y = __fdividef(v, 1.f + __expf(-v));
+  return v < -87.f ? 0.f : y;
+}
+
+// --------------------------------------------------------------- sequences
+// Rows [begin, end) of one sequence; begin > end marks a bad pair of offsets.
+struct Span {
+  int begin, end;
+};
+
+struct Sequences {
+  const int* offsets;  // device [n + 1], or nullptr: every sequence has ``length`` rows
+  const int* codes;    // device [n], or nullptr: no states
+  int n, length, rows, num_slots;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ Span span_of(const Sequences& q, int s) {
+  if (!q.offsets) return {s * q.length, (s + 1) * q.length};
+  const int b = q.offsets[s], e = q.offsets[s + 1];
+  return b >= 0 && b <= e && e <= q.rows ? Span{b, e} : Span{1, 0};
+}
+
+// The last sequence that begins at or before row r (offsets increase), -1 if
+// none does. Any content of ``offsets`` gives an index below n.
+__device__ __forceinline__ int sequence_at(const Sequences& q, int r) {
+  if (!q.offsets) return r / q.length;
+  int lo = -1, hi = q.n - 1;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (q.offsets[mid] <= r)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// A sequence's slot: where its state is read (table < 0: a fresh start, from
+// zeros) and where the advanced state goes. slot < 0: no state, or a code
+// outside the pool (recorded).
+struct SlotRef {
+  int slot, read, write;
+  bool bad;
+};
+
+__device__ __forceinline__ SlotRef slot_of(const Sequences& q, int s) {
+  if (!q.codes) return {-1, -1, -1, false};
+  const int code = q.codes[s], slot = code >> 2;
+  if (slot < 0 || slot >= q.num_slots) {
+    record_error(q.status, kDevBadSlot);
+    return {-1, -1, -1, true};
+  }
+  return {slot, code & 2 ? -1 : code & 1, (code & 1) ^ 1, false};
+}
+
+// ------------------------------------------------------------ host helpers
+inline bool aligned_for(const void* p, long long stride, int elem, int width) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % (size_t)(elem * width) == 0 && stride % width == 0);
+}
+
+inline int elem_bytes(int type) { return type == FAV_TYPE_F32 ? 4 : 2; }
+
+// Launches that follow one another in a stream overlap (see launch_overlapped).
+template <typename Args>
+inline cudaError_t launch_op(void (*kernel)(Args), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
+                             const Args& a, unsigned cluster = 1) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) cudaGetLastError();  // reported here: clear it for the caller's next call
+  return e;
+}
+
+}  // namespace fav

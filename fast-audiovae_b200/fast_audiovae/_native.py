@@ -21,8 +21,33 @@ NUM_COEFFICIENTS = 188
 STATUS = {0: "FAV_OK", 1: "FAV_INVALID_ARGUMENT", 2: "FAV_UNSUPPORTED", 3: "FAV_OVERLAP",
           4: "FAV_SIZE_OVERFLOW", 5: "FAV_DEVICE_ERROR", 6: "FAV_TIMEOUT"}
 
-# Every symbol the header declares, with its ctypes signature.
 _P = ct.c_void_p
+
+
+def _struct(name, fields):
+    """A ctypes structure from ``"type: name name ..."`` lines in the header's order."""
+    kinds = {"ptr": ct.c_void_p, "i64": ct.c_int64, "size": ct.c_size_t, "f32": ct.c_float, "i32": ct.c_int32}
+    return type(name, (ct.Structure,), {"_fields_": [
+        (field, kinds[kind]) for kind, _, names in (line.partition(":") for line in fields)
+        for field in names.split()]})
+
+
+# Argument structures of the stream operators (fav_conv_args and so on).
+ConvArgs = _struct("ConvArgs", [
+    "ptr: x y", "i64: x_stride y_stride", "ptr: weight bias state_pool slot_codes offsets status",
+    "i32: type channels taps activation n length rows num_slots"])
+ScanArgs = _struct("ScanArgs", [
+    "ptr: x dt z b c y",
+    "i64: x_stride dt_stride z_stride b_stride b_group_stride c_stride c_group_stride y_stride",
+    "ptr: a d dt_bias state_pool slot_codes offsets status workspace", "size: workspace_bytes",
+    "i32: type channels states groups softplus n length rows num_slots"])
+NormArgs = _struct("NormArgs", [
+    "ptr: x y", "i64: x_stride y_stride", "ptr: weight bias alpha reciprocal offsets status", "f32: eps",
+    "i32: type channels groups activation n length rows"])
+Int4Args = _struct("Int4Args", [
+    "ptr: x y", "i64: x_stride y_stride", "ptr: weight scales bias", "i32: type rows depth out group"])
+
+# Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "fav_abi_version": ([], ct.c_int32),
     "fav_last_error": ([], ct.c_char_p),
@@ -49,6 +74,11 @@ SIGNATURES = {
                                ct.c_int32, ct.POINTER(ct.c_void_p), _P], ct.c_int32),
     "fav_debug_step_gated": ([_P, _P, ct.c_int32, _P, ct.c_int32, ct.c_int32, _P, _P, _P, ct.c_size_t, _P,
                               ct.c_int32, ct.c_uint32, _P, _P], ct.c_int32),
+    "fav_causal_conv": ([ct.POINTER(ConvArgs), _P], ct.c_int32),
+    "fav_selective_scan": ([ct.POINTER(ScanArgs), _P], ct.c_int32),
+    "fav_selective_scan_workspace_bytes": ([ct.POINTER(ScanArgs)], ct.c_size_t),
+    "fav_group_norm": ([ct.POINTER(NormArgs), _P], ct.c_int32),
+    "fav_project_int4": ([ct.POINTER(Int4Args), _P], ct.c_int32),
     "fav_test_gemm": ([_P, ct.c_int32, ct.c_int32, _P, ct.c_int32, ct.c_int32, _P, _P], ct.c_int32),
     "fav_test_sine": ([_P, ct.c_int32, _P, _P], ct.c_int32),
 }

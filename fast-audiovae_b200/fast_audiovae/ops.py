@@ -1,0 +1,425 @@
+"""Stream operators on device tensors: the layers of a recurrent latent model.
+
+The decoder turns latents into audio, one 40 ms frame of every stream a step.
+These are the operators of a model that makes those latents the same way, in
+the decoder's own terms: channels-last rows, one call for all streams, a
+fixed-size state per stream in a slot of a pool, transactional slot codes.
+
+* ``causal_conv``: short causal depthwise convolution with a carried history;
+* ``selective_scan``: selective state space scan with carried states;
+* ``group_norm``: group norm with SiLU or the decoder's Snake;
+* ``project_int4``: projection by 4-bit weights with group scales.
+
+Rows and sequences. Arrays are torch tensors on one CUDA device (fp32, bf16 or
+fp16, adjacent channels, any row stride):
+
+* ``[rows, channels]`` alone: a decoding step, every row a stream of its own;
+* ``[n, length, channels]``: n sequences of one length;
+* ``[rows, channels]`` with ``offsets`` (int32 ``[n + 1]`` on the device):
+  packed sequences, sequence i in rows ``offsets[i]:offsets[i + 1]``, empty
+  ones among them. Rows of no sequence keep what ``out`` held.
+
+States. A state tensor is ``[slots, 2, ...]``: two tables per slot.
+``codes`` (int32 ``[n]`` on the device, see ``StreamSlots``) name the table a
+sequence reads and whether it starts afresh; the advanced state goes to the
+other table, so a step that is not committed has changed nothing.
+
+``status`` is an optional int32 tensor of one element, zero before the call:
+0x201 after it means offsets that decrease or leave the rows (the call's
+outputs are then undefined), 0x202 a code outside the pool (its sequence is
+skipped). Without it the same happens silently; either way no memory outside
+the arrays is touched.
+
+Coefficients are contiguous fp32; sums, states and statistics run in fp32, and
+every output is rounded once to its type. Work is enqueued on the current
+stream of the tensors' device without synchronising and may be captured in a
+CUDA graph. The operators are for inference and have no gradients. They run in
+``libfav_cuda.so``; there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as ct
+
+import numpy as np
+import torch
+
+from . import _native
+from ._native import ConvArgs, Int4Args, NormArgs, ScanArgs
+
+__all__ = ["causal_conv", "selective_scan", "group_norm", "project_int4", "quantize_int4", "conv_state",
+           "scan_state", "StreamSlots"]
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTIVATIONS = {None: 0, "silu": 1, "snake": 2}
+_I32, _F32 = torch.int32, torch.float32
+_FRESH = 2
+_lib = None
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _library(device):
+    """The native library, for tensors on ``device``."""
+    global _lib
+    if device.type != "cuda":
+        raise RuntimeError("Stream operators run on CUDA tensors; there is no CPU path")
+    if _lib is None:
+        _lib = _native.load_library()
+    return _lib
+
+
+def _call(lib, function, args, device):
+    """Run a C-ABI operator on the current stream of ``device``."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = function(ct.byref(args), _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = function(ct.byref(args), _raw_stream(index))
+    if status:
+        _native.check(lib, status)
+
+
+def _main(x):
+    """Checks an operator's first argument; returns its type code and device."""
+    kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if kind is None:
+        raise ValueError("x must be a float32, bfloat16 or float16 tensor")
+    return kind, x.device
+
+
+def _graph_free(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("Stream operators have no gradients; call them under torch.no_grad()")
+
+
+def _array(t, name, like, shape):
+    """Address and row stride of an array of ``like``'s type with adjacent channels."""
+    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
+        raise ValueError(f"{name} must be a {like.dtype} tensor of shape {list(shape)} on {like.device}")
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] != 1:
+        raise ValueError(f"{name} must have adjacent channels (stride 1)")
+    return t.data_ptr(), _row_stride(name, shape, strides, shape[-1])
+
+
+def _row_stride(name, shape, strides, width):
+    """The one stride between rows of ``[rows, ...]`` or ``[n, length, ...]``."""
+    lead = len(shape) - (1 if width is not None else 2)
+    if lead == 1:
+        return strides[0] if shape[0] != 1 or width is None else width
+    if shape[1] == 1:
+        return strides[0]
+    if shape[0] != 1 and strides[0] != shape[1] * strides[1]:
+        raise ValueError(f"{name} must have one stride between all its rows")
+    return strides[1]
+
+
+def _vector(t, name, like, shape):
+    """Address of a contiguous fp32 coefficient array (0 for None)."""
+    if t is None:
+        return 0
+    if (not isinstance(t, torch.Tensor) or t.dtype != _F32 or t.device != like.device or t.shape != shape
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {list(shape)} on {like.device}")
+    return t.data_ptr()
+
+
+def _index(t, name, like, count):
+    if (not isinstance(t, torch.Tensor) or t.dtype != _I32 or t.device != like.device or t.dim() != 1
+            or not t.is_contiguous() or (count is not None and t.shape[0] != count)):
+        raise ValueError(f"{name} must be a contiguous int32 tensor"
+                         f"{'' if count is None else f' of {count} elements'} on {like.device}")
+    return t.data_ptr()
+
+
+def _sequences(x, offsets):
+    """(sequences, length, rows, offsets address) of ``x``; length 0 with offsets."""
+    dims = x.dim()
+    if offsets is not None:
+        if dims != 2:
+            raise ValueError("Packed sequences (offsets) require x of shape [rows, channels]")
+        address = _index(offsets, "offsets", x, None)
+        if offsets.shape[0] < 1:
+            raise ValueError("offsets must hold n + 1 elements")
+        return offsets.shape[0] - 1, 0, x.shape[0], address
+    if dims == 2:
+        return x.shape[0], 1, x.shape[0], 0
+    if dims == 3:
+        if x.shape[1] < 1:
+            raise ValueError("Sequences without offsets must have at least one row")
+        return x.shape[0], x.shape[1], x.shape[0] * x.shape[1], 0
+    raise ValueError("x must have shape [rows, channels] or [n, length, channels]")
+
+
+def _states(state, codes, x, n, shape, dtype):
+    """Addresses of a state pool and its codes, and its slots (0s for None)."""
+    if state is None and codes is None:
+        return 0, 0, 0
+    if state is None or codes is None:
+        raise ValueError("state and codes go together")
+    if (not isinstance(state, torch.Tensor) or state.dtype != dtype or state.device != x.device
+            or state.shape[1:] != shape or not state.is_contiguous()):
+        raise ValueError(f"state must be a contiguous {dtype} tensor of shape {['slots', *shape]} on {x.device}")
+    if state.shape[0] < n:
+        raise ValueError(f"{n} sequences need at least as many slots; state has {state.shape[0]}")
+    return state.data_ptr(), _index(codes, "codes", x, n), state.shape[0]
+
+
+def _status(status, x):
+    return 0 if status is None else _index(status, "status", x, 1)
+
+
+def _output(out, x):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+
+
+def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=None, codes=None, status=None, out=None):
+    """Causal depthwise convolution over each sequence's rows, 2 to 8 taps.
+
+    ``y[t, c] = act(bias[c] + sum_j weight[c, j] * x[t - (taps - 1) + j, c])``
+    with ``weight`` ``[channels, taps]`` (the last tap meets the newest row),
+    ``bias`` ``[channels]`` and ``activation`` None or ``"silu"``. Rows before a
+    sequence's first come from ``state`` ``[slots, 2, taps - 1, channels]`` (x's
+    type, oldest first; ``conv_state`` makes one) or are zero.
+    """
+    kind, device = _main(x)
+    _graph_free(x, weight, bias)
+    n, length, rows, offsets_at = _sequences(x, offsets)
+    channels = x.shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
+        raise ValueError("weight must have shape [channels, taps] with 2 to 8 taps")
+    if activation not in (None, "silu"):
+        raise ValueError("activation must be None or 'silu'")
+    taps = weight.shape[1]
+    weight_at = _vector(weight, "weight", x, (channels, taps))
+    bias_at = _vector(bias, "bias", x, (channels,))
+    x_at, x_stride = _array(x, "x", x, x.shape)
+    pool_at, codes_at, slots = _states(state, codes, x, n, (2, taps - 1, channels), x.dtype)
+    status_at = _status(status, x)
+    lib = _library(device)
+    out = _output(out, x)
+    y_at, y_stride = _array(out, "out", x, x.shape)
+    if n:
+        _call(lib, lib.fav_causal_conv,
+              ConvArgs(x_at, y_at, x_stride, y_stride, weight_at, bias_at, pool_at, codes_at, offsets_at, status_at,
+                       kind, channels, taps, _ACTIVATIONS[activation], n, length, rows, slots), device)
+    return out
+
+
+def _maps(t, name, x, lead, groups, states):
+    """Address, row stride and group stride of an input or output map."""
+    if (not isinstance(t, torch.Tensor) or t.dtype != x.dtype or t.device != x.device
+            or t.shape[:-2] != lead or t.shape[-2:] != (groups, states)):
+        raise ValueError(f"{name} must be a {x.dtype} tensor of shape {[*lead, groups, states]} on {x.device}")
+    strides = t.stride()
+    if strides[-1] != 1 and states != 1:
+        raise ValueError(f"{name} must have adjacent states (stride 1)")
+    return t.data_ptr(), _row_stride(name, t.shape, strides, None), strides[-2] if groups > 1 else 0
+
+
+def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=True, offsets=None, state=None,
+                   codes=None, status=None, out=None):
+    """Selective state space scan over each sequence's rows.
+
+    Channel c of group g keeps N states; ``delta = softplus(dt + dt_bias)`` (or
+    the sum itself), and row by row
+
+    ``h[n, c] = exp(delta * a[n, c]) * h[n, c] + delta * x[t, c] * b[t, g, n]``
+    ``y[t, c] = (sum_n c[t, g, n] * h[n, c] + d[c] * x[t, c]) * silu(z[t, c])``
+
+    ``dt`` and ``z`` are shaped like ``x``; ``b`` and ``c`` are
+    ``[..., groups, N]`` over the same rows (groups divide the channels); ``a``
+    is ``[N, channels]`` and ``d`` and ``dt_bias`` are ``[channels]``. N is 1 to
+    128. ``state`` is ``[slots, 2, N, channels]`` fp32 (``scan_state``).
+    """
+    kind, device = _main(x)
+    _graph_free(x, dt, a, b, c, d, z, dt_bias)
+    n, length, rows, offsets_at = _sequences(x, offsets)
+    shape = x.shape
+    channels = shape[-1]
+    if not isinstance(a, torch.Tensor) or a.dim() != 2 or not 1 <= a.shape[0] <= 128:
+        raise ValueError("a must have shape [states, channels] with 1 to 128 states")
+    states = a.shape[0]
+    if not isinstance(b, torch.Tensor) or b.dim() != x.dim() + 1 or b.shape[-2] < 1 or channels % b.shape[-2]:
+        raise ValueError("b must have shape [..., groups, states] with groups that divide the channels")
+    groups = b.shape[-2]
+    x_at, x_stride = _array(x, "x", x, shape)
+    dt_at, dt_stride = _array(dt, "dt", x, shape)
+    z_at, z_stride = _array(z, "z", x, shape) if z is not None else (0, 0)
+    b_at, b_stride, b_group = _maps(b, "b", x, shape[:-1], groups, states)
+    c_at, c_stride, c_group = _maps(c, "c", x, shape[:-1], groups, states)
+    a_at = _vector(a, "a", x, (states, channels))
+    d_at = _vector(d, "d", x, (channels,))
+    bias_at = _vector(dt_bias, "dt_bias", x, (channels,))
+    pool_at, codes_at, slots = _states(state, codes, x, n, (2, states, channels), _F32)
+    status_at = _status(status, x)
+    lib = _library(device)
+    out = _output(out, x)
+    y_at, y_stride = _array(out, "out", x, shape)
+    if not n:
+        return out
+    args = ScanArgs(x_at, dt_at, z_at, b_at, c_at, y_at, x_stride, dt_stride, z_stride, b_stride, b_group, c_stride,
+                    c_group, y_stride, a_at, d_at, bias_at, pool_at, codes_at, offsets_at, status_at, 0, 0, kind,
+                    channels, states, groups, bool(softplus), n, length, rows, slots)
+    if length != 1:
+        need = lib.fav_selective_scan_workspace_bytes(ct.byref(args))
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    _call(lib, lib.fav_selective_scan, args, device)
+    return out
+
+
+def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, alpha=None, reciprocal=None,
+               offsets=None, status=None, out=None):
+    """Group norm with an activation, channels last.
+
+    ``y = act((x - mean) / sqrt(variance + eps) * weight + bias)`` with the mean
+    and the biased variance over a sequence's rows and the neighbouring
+    ``channels / groups`` channels of a group; of ``[rows, channels]`` without
+    ``offsets`` every row is normalised by itself, as a step needs it.
+    ``activation`` is None, ``"silu"`` or ``"snake"``, the decoder's
+    ``v + reciprocal * sin(alpha * v)**2`` with ``[channels]`` coefficients.
+    """
+    kind, device = _main(x)
+    _graph_free(x, weight, bias, alpha, reciprocal)
+    n, length, rows, offsets_at = _sequences(x, offsets)
+    channels = x.shape[-1]
+    if type(groups) is not int or groups < 1 or channels % groups:
+        raise ValueError("groups must be a positive int that divides the channels")
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be None, 'silu' or 'snake'")
+    if (activation == "snake") != (alpha is not None) or (activation == "snake") != (reciprocal is not None):
+        raise ValueError("alpha and reciprocal belong to activation='snake'")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    shape = (channels,)
+    coefficients = (_vector(weight, "weight", x, shape), _vector(bias, "bias", x, shape),
+                    _vector(alpha, "alpha", x, shape), _vector(reciprocal, "reciprocal", x, shape))
+    x_at, x_stride = _array(x, "x", x, x.shape)
+    status_at = _status(status, x)
+    lib = _library(device)
+    out = _output(out, x)
+    y_at, y_stride = _array(out, "out", x, x.shape)
+    if n:
+        _call(lib, lib.fav_group_norm,
+              NormArgs(x_at, y_at, x_stride, y_stride, *coefficients, offsets_at, status_at, eps, kind, channels,
+                       groups, _ACTIVATIONS[activation], n, length, rows), device)
+    return out
+
+
+def project_int4(x, weight, scales, bias=None, *, group, out=None):
+    """Rows times 4-bit weights: ``y = x @ w.T + bias`` for the rows of a step.
+
+    ``w[r, k] = (q[r, k] - 8) * scales[r, k // group]`` with ``q`` in 0..15, two
+    to a byte along k, the even k in the low half: ``weight`` is uint8
+    ``[out, depth / 2]``, ``scales`` fp32 ``[out, ceil(depth / group)]``
+    (``quantize_int4`` makes both), ``x`` ``[rows, depth]``. ``group`` and the
+    depth are multiples of 32.
+    """
+    kind, device = _main(x)
+    _graph_free(x, scales, bias)
+    if x.dim() != 2:
+        raise ValueError("x must have shape [rows, depth]")
+    rows, depth = x.shape
+    if type(group) is not int or group < 32 or group % 32 or depth < 32 or depth % 32:
+        raise ValueError("group and the depth must be positive multiples of 32")
+    if (not isinstance(weight, torch.Tensor) or weight.dtype != torch.uint8 or weight.device != device
+            or weight.dim() != 2 or weight.shape[1] != depth // 2 or not weight.is_contiguous()):
+        raise ValueError(f"weight must be a contiguous uint8 tensor of shape ['out', {depth // 2}] on {device}")
+    if weight.data_ptr() % 16:
+        raise ValueError("weight must be 16-byte aligned")
+    width = weight.shape[0]
+    if scales is None:
+        raise ValueError("scales are required")
+    scales_at = _vector(scales, "scales", x, (width, -(-depth // group)))
+    bias_at = _vector(bias, "bias", x, (width,))
+    x_at, x_stride = _array(x, "x", x, x.shape)
+    lib = _library(device)
+    out = torch.empty((rows, width), dtype=x.dtype, device=device) if out is None else out
+    y_at, y_stride = _array(out, "out", x, (rows, width))
+    if rows and width:
+        _call(lib, lib.fav_project_int4,
+              Int4Args(x_at, y_at, x_stride, y_stride, weight.data_ptr(), scales_at, bias_at, kind, rows, depth, width,
+                       group), device)
+    return out
+
+
+def quantize_int4(weight, group):
+    """4-bit codes and group scales of ``weight`` ``[out, depth]`` for ``project_int4``.
+
+    Symmetric: a group's scale is its largest magnitude over 7 (1 for a group of
+    zeros), codes round to nearest, ties to even.
+    """
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError("weight must be a floating point tensor of shape [out, depth]")
+    width, depth = weight.shape
+    if type(group) is not int or group < 32 or group % 32 or depth < 32 or depth % 32:
+        raise ValueError("group and the depth must be positive multiples of 32")
+    groups = -(-depth // group)
+    w = torch.zeros((width, groups * group), dtype=_F32, device=weight.device)
+    w[:, :depth] = weight
+    w = w.view(width, groups, group)
+    scales = w.abs().amax(2) / 7
+    if not torch.isfinite(scales).all():
+        raise ValueError("weight must contain only finite values")
+    scales[scales == 0] = 1
+    q = (torch.round(w / scales[:, :, None]).clamp(-7, 7) + 8).to(torch.uint8).view(width, -1)[:, :depth]
+    return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), scales.contiguous()
+
+
+def conv_state(slots, channels, taps, *, dtype=torch.bfloat16, device="cuda"):
+    """A zeroed state pool of ``causal_conv``."""
+    return torch.zeros((slots, 2, taps - 1, channels), dtype=dtype, device=device)
+
+
+def scan_state(slots, channels, states, *, device="cuda"):
+    """A zeroed state pool of ``selective_scan``."""
+    return torch.zeros((slots, 2, states, channels), dtype=_F32, device=device)
+
+
+class StreamSlots:
+    """Read tables and fresh starts of a pool's slots, as the decoder keeps its own.
+
+    One ``StreamSlots`` serves every layer of a model, since all layers of a
+    step advance together: ``codes(slots)`` before the step, and
+    ``commit(slots)`` once it has succeeded. A step that is not committed
+    leaves every state as it was. Slots start afresh until their first commit
+    and again after ``reset``.
+    """
+
+    def __init__(self, slots, *, device="cuda"):
+        if type(slots) is not int or slots < 1:
+            raise ValueError("slots must be a positive int")
+        self.device = torch.device(device)
+        self._table = np.zeros(slots, np.int32)
+        self._fresh = np.ones(slots, np.int32)
+
+    def _checked(self, slots):
+        index = np.asarray(slots)
+        if index.size == 0:
+            index = index.astype(np.int64)
+        if index.ndim != 1 or index.dtype.kind not in "iu":
+            raise ValueError("slots must be a sequence of ints")
+        if index.size and (index.min() < 0 or index.max() >= len(self._table)):
+            raise ValueError(f"slots must lie in [0, {len(self._table)})")
+        if len(np.unique(index)) != index.size:
+            raise ValueError("A slot may appear only once per step")
+        return index
+
+    def codes(self, slots):
+        """The slot codes of a step over distinct ``slots``, on the device."""
+        index = self._checked(slots)
+        codes = (index.astype(np.int32) << 2) | (self._fresh[index] * _FRESH) | self._table[index]
+        return torch.from_numpy(codes).to(self.device)
+
+    def commit(self, slots):
+        index = self._checked(slots)
+        self._table[index] ^= 1
+        self._fresh[index] = 0
+
+    def reset(self, slots):
+        self._fresh[self._checked(slots)] = 1

@@ -249,6 +249,123 @@ FAV_API int32_t fav_test_gemm(const float *a, int32_t m, int32_t k, const float 
  * Asynchronous on cuda_stream. */
 FAV_API int32_t fav_test_sine(const float *x, int32_t n, float *out, void *cuda_stream);
 
+/* ---------------------------------------------------------------------------
+ * Stream operators. The reference has no counterpart: they are the layers of a
+ * recurrent model that makes latents for many streams, one 40 ms frame a step,
+ * in this library's own terms (channels-last rows, caller-owned buffers, state
+ * pools with two tables a slot, slot codes, a device status word).
+ *
+ * Rows and sequences. Arrays are [rows][channels] with a row stride in
+ * elements and adjacent channels. `offsets` (device int32[n + 1]) gives
+ * sequence i the rows offsets[i] .. offsets[i + 1]; a sequence may have none,
+ * and rows before the first or behind the last are left as they are. With
+ * NULL offsets every sequence has `length` rows (rows = n * length); length 1
+ * is a decoding step, one row per stream.
+ *
+ * States. A pool holds two tables per slot; slot_codes (device int32[n]) are
+ * (slot << 2) | (fresh << 1) | read_table, as in fav_step: a sequence reads
+ * table read_table of its slot, or zeros with fresh = 1, and its advanced
+ * state goes to the other table (of an empty sequence: the state as it was).
+ * Slots in one call must be distinct. NULL state_pool and slot_codes: zero
+ * history, nothing kept.
+ *
+ * Status. `status` (device uint32, 0 on entry, may be NULL) receives 0x201
+ * when offsets decrease or leave the rows (the outputs are then undefined) and
+ * 0x202 when a slot code lies outside the pool (its sequence is skipped, its
+ * outputs not written); neither touches memory outside the arrays.
+ *
+ * Coefficients are fp32. Sums, states and statistics are fp32; each output is
+ * rounded once to `type`. Calls enqueue on `cuda_stream` of the current
+ * device, allocate nothing and may be captured. Outputs must not overlap
+ * inputs (FAV_OVERLAP). */
+typedef enum fav_type { FAV_TYPE_F32 = 0, FAV_TYPE_BF16 = 1, FAV_TYPE_F16 = 2 } fav_type;
+typedef enum fav_activation {
+  FAV_ACTIVATION_NONE = 0,
+  FAV_ACTIVATION_SILU = 1, /* v / (1 + e^-v) */
+  FAV_ACTIVATION_SNAKE = 2 /* v + reciprocal * sin(alpha * v)^2, the decoder's */
+} fav_activation;
+
+/* Causal depthwise convolution with `taps` (2..8) rows and an optional SiLU:
+ *   y[t][c] = act(bias[c] + sum_j weight[c][j] * x[t - (taps - 1) + j][c]).
+ * state_pool: [num_slots][2][taps - 1][channels] of `type`, the latest inputs,
+ * oldest first. bias may be NULL. */
+typedef struct fav_conv_args {
+  const void *x;
+  void *y;
+  int64_t x_stride, y_stride;
+  const float *weight; /* [channels][taps] */
+  const float *bias;   /* [channels] or NULL */
+  void *state_pool;
+  const int32_t *slot_codes;
+  const int32_t *offsets;
+  uint32_t *status;
+  int32_t type, channels, taps, activation, n, length, rows, num_slots;
+} fav_conv_args;
+FAV_API int32_t fav_causal_conv(const fav_conv_args *args, void *cuda_stream);
+
+/* Selective state space scan, N = `states` (1..128) states a channel; channel
+ * c belongs to group c / (channels / groups):
+ *   delta   = softplus(dt[t][c] + dt_bias[c])   (softplus = 0: the sum itself)
+ *   h[n][c] = exp(delta * a[n][c]) * h[n][c] + delta * x[t][c] * b[t][g][n]
+ *   y[t][c] = (sum_n c[t][g][n] * h[n][c] + d[c] * x[t][c]) * silu(z[t][c])
+ * x, dt, z, y: [rows][channels]; b, c: [rows][groups][N] with row and group
+ * strides; a: [N][channels]. state_pool: [num_slots][2][N][channels] fp32.
+ * z, d and dt_bias may be NULL. Long sequences that are too few to fill the
+ * GPU are cut into pieces, whose states need `workspace`
+ * (fav_selective_scan_workspace_bytes, which reads sizes only; 0 for a step). */
+typedef struct fav_scan_args {
+  const void *x, *dt, *z, *b, *c;
+  void *y;
+  int64_t x_stride, dt_stride, z_stride, b_stride, b_group_stride, c_stride, c_group_stride, y_stride;
+  const float *a;       /* [states][channels] */
+  const float *d;       /* [channels] or NULL */
+  const float *dt_bias; /* [channels] or NULL */
+  float *state_pool;
+  const int32_t *slot_codes;
+  const int32_t *offsets;
+  uint32_t *status;
+  void *workspace;
+  size_t workspace_bytes;
+  int32_t type, channels, states, groups, softplus, n, length, rows, num_slots;
+} fav_scan_args;
+FAV_API size_t fav_selective_scan_workspace_bytes(const fav_scan_args *args);
+FAV_API int32_t fav_selective_scan(const fav_scan_args *args, void *cuda_stream);
+
+/* Group norm with an activation, over channels-last rows: per sequence and
+ * group of channels / groups neighbouring channels,
+ *   y = act((x - mean) / sqrt(variance + eps) * weight[c] + bias[c])
+ * with the mean and (biased) variance over the sequence's rows and the group's
+ * channels. length = 1 without offsets normalises every row by itself.
+ * weight and bias may be NULL (1 and 0); alpha and reciprocal [channels] are
+ * required by FAV_ACTIVATION_SNAKE. */
+typedef struct fav_norm_args {
+  const void *x;
+  void *y;
+  int64_t x_stride, y_stride;
+  const float *weight, *bias, *alpha, *reciprocal;
+  const int32_t *offsets;
+  uint32_t *status;
+  float eps;
+  int32_t type, channels, groups, activation, n, length, rows;
+} fav_norm_args;
+FAV_API int32_t fav_group_norm(const fav_norm_args *args, void *cuda_stream);
+
+/* Projection by 4-bit weights with group scales, for the few rows of a step:
+ *   y[m][r] = bias[r] + sum_k x[m][k] * (q[r][k] - 8) * scales[r][k / group],
+ * q in 0..15, two to a byte along k, the even k in the low half: weight
+ * [out][depth / 2]. scales: [out][ceil(depth / group)]. group and depth are
+ * multiples of 32. bias may be NULL. */
+typedef struct fav_int4_args {
+  const void *x;
+  void *y;
+  int64_t x_stride, y_stride;
+  const uint8_t *weight;
+  const float *scales;
+  const float *bias;
+  int32_t type, rows, depth, out, group;
+} fav_int4_args;
+FAV_API int32_t fav_project_int4(const fav_int4_args *args, void *cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
