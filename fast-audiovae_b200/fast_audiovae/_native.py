@@ -5,6 +5,7 @@ Loading never falls back to anything: a missing or unloadable library raises.
 from __future__ import annotations
 
 import ctypes as ct
+import struct as pack
 import threading
 from pathlib import Path
 
@@ -32,6 +33,15 @@ def _struct(name, fields):
         for field in names.split()]})
 
 
+def _packer(struct):
+    """``struct``'s C image from its fields' values in order, as bytes a call can be given (a
+    third of the time that a ctypes structure takes to fill)."""
+    letters = {ct.c_void_p: "P", ct.c_int64: "q", ct.c_size_t: "N", ct.c_float: "f", ct.c_int32: "i"}
+    image = pack.Struct("@" + "".join(letters[kind] for _, kind in struct._fields_) + "0P")
+    assert image.size == ct.sizeof(struct)
+    return image.pack
+
+
 # Argument structures of the stream operators (fav_conv_args and so on).
 ConvArgs = _struct("ConvArgs", [
     "ptr: x y", "i64: x_stride y_stride", "ptr: weight bias state_pool slot_codes offsets status",
@@ -46,6 +56,8 @@ NormArgs = _struct("NormArgs", [
     "i32: type channels groups activation n length rows"])
 Int4Args = _struct("Int4Args", [
     "ptr: x y", "i64: x_stride y_stride", "ptr: weight scales bias", "i32: type rows depth out group"])
+
+CONV_ARGS, SCAN_ARGS, NORM_ARGS, INT4_ARGS = map(_packer, (ConvArgs, ScanArgs, NormArgs, Int4Args))
 
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
@@ -74,11 +86,11 @@ SIGNATURES = {
                                ct.c_int32, ct.POINTER(ct.c_void_p), _P], ct.c_int32),
     "fav_debug_step_gated": ([_P, _P, ct.c_int32, _P, ct.c_int32, ct.c_int32, _P, _P, _P, ct.c_size_t, _P,
                               ct.c_int32, ct.c_uint32, _P, _P], ct.c_int32),
-    "fav_causal_conv": ([ct.POINTER(ConvArgs), _P], ct.c_int32),
-    "fav_selective_scan": ([ct.POINTER(ScanArgs), _P], ct.c_int32),
-    "fav_selective_scan_workspace_bytes": ([ct.POINTER(ScanArgs)], ct.c_size_t),
-    "fav_group_norm": ([ct.POINTER(NormArgs), _P], ct.c_int32),
-    "fav_project_int4": ([ct.POINTER(Int4Args), _P], ct.c_int32),
+    "fav_causal_conv": ([_P, _P], ct.c_int32),
+    "fav_selective_scan": ([_P, _P], ct.c_int32),
+    "fav_selective_scan_workspace_bytes": ([_P], ct.c_size_t),
+    "fav_group_norm": ([_P, _P], ct.c_int32),
+    "fav_project_int4": ([_P, _P], ct.c_int32),
     "fav_test_gemm": ([_P, ct.c_int32, ct.c_int32, _P, ct.c_int32, ct.c_int32, _P, _P], ct.c_int32),
     "fav_test_sine": ([_P, ct.c_int32, _P, _P], ct.c_int32),
 }

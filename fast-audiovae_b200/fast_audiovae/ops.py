@@ -38,13 +38,11 @@ CUDA graph. The operators are for inference and have no gradients. They run in
 """
 from __future__ import annotations
 
-import ctypes as ct
-
 import numpy as np
 import torch
 
 from . import _native
-from ._native import ConvArgs, Int4Args, NormArgs, ScanArgs
+from ._native import CONV_ARGS, INT4_ARGS, NORM_ARGS, SCAN_ARGS
 
 __all__ = ["causal_conv", "selective_scan", "group_norm", "project_int4", "quantize_int4", "conv_state",
            "scan_state", "StreamSlots"]
@@ -54,62 +52,68 @@ _ACTIVATIONS = {None: 0, "silu": 1, "snake": 2}
 _I32, _F32 = torch.int32, torch.float32
 _FRESH = 2
 _lib = None
+_grad_enabled = torch.is_grad_enabled
+_current_device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _library(device):
-    """The native library, for tensors on ``device``."""
+def _library(index):
+    """The native library, for tensors on CUDA device ``index`` (negative: the CPU)."""
     global _lib
-    if device.type != "cuda":
+    if index < 0:
         raise RuntimeError("Stream operators run on CUDA tensors; there is no CPU path")
     if _lib is None:
         _lib = _native.load_library()
     return _lib
 
 
-def _call(lib, function, args, device):
-    """Run a C-ABI operator on the current stream of ``device``."""
-    index = device.index
-    if torch.cuda.current_device() == index:
-        status = function(ct.byref(args), _raw_stream(index))
+def _call(lib, function, args, index):
+    """Run a C-ABI operator on the current stream of device ``index``."""
+    if _current_device() == index:
+        status = function(args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = function(ct.byref(args), _raw_stream(index))
+            status = function(args, _raw_stream(index))
     if status:
         _native.check(lib, status)
 
 
+# The checks below run on every call of a step that takes microseconds, so they
+# read each tensor attribute once. One that is missing is a ValueError too.
 def _main(x):
-    """Checks an operator's first argument; returns its type code and device."""
-    kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
-    if kind is None:
-        raise ValueError("x must be a float32, bfloat16 or float16 tensor")
-    return kind, x.device
+    """Checks an operator's first argument; returns its type code and device index."""
+    try:
+        return _TYPES[x.dtype], x.get_device()
+    except (AttributeError, KeyError, TypeError):
+        raise ValueError("x must be a float32, bfloat16 or float16 tensor") from None
 
 
 def _graph_free(*tensors):
-    if torch.is_grad_enabled():
+    if _grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("Stream operators have no gradients; call them under torch.no_grad()")
 
 
-def _array(t, name, like, shape):
-    """Address and row stride of an array of ``like``'s type with adjacent channels."""
-    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
-        raise ValueError(f"{name} must be a {like.dtype} tensor of shape {list(shape)} on {like.device}")
+def _array(t, name, dtype, index, shape):
+    """Address and row stride of an array of x's type with adjacent channels."""
+    try:
+        good = t.dtype is dtype and t.get_device() == index and t.shape == shape
+    except AttributeError:
+        good = False
+    if not good:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)} on x's device")
     strides = t.stride()
     if strides[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"{name} must have adjacent channels (stride 1)")
-    return t.data_ptr(), _row_stride(name, shape, strides, shape[-1])
+    if len(shape) == 2:
+        return t.data_ptr(), strides[0] if shape[0] != 1 else shape[1]
+    return t.data_ptr(), _row_stride(name, shape, strides)
 
 
-def _row_stride(name, shape, strides, width):
-    """The one stride between rows of ``[rows, ...]`` or ``[n, length, ...]``."""
-    lead = len(shape) - (1 if width is not None else 2)
-    if lead == 1:
-        return strides[0] if shape[0] != 1 or width is None else width
+def _row_stride(name, shape, strides):
+    """The one stride between the rows of ``[n, length, ...]``."""
     if shape[1] == 1:
         return strides[0]
     if shape[0] != 1 and strides[0] != shape[1] * strides[1]:
@@ -117,63 +121,61 @@ def _row_stride(name, shape, strides, width):
     return strides[1]
 
 
-def _vector(t, name, like, shape):
+def _vector(t, name, index, shape):
     """Address of a contiguous fp32 coefficient array (0 for None)."""
     if t is None:
         return 0
-    if (not isinstance(t, torch.Tensor) or t.dtype != _F32 or t.device != like.device or t.shape != shape
-            or not t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {list(shape)} on {like.device}")
-    return t.data_ptr()
+    try:
+        if t.dtype is _F32 and t.get_device() == index and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    raise ValueError(f"{name} must be a contiguous float32 tensor of shape {list(shape)} on x's device")
 
 
-def _index(t, name, like, count):
-    if (not isinstance(t, torch.Tensor) or t.dtype != _I32 or t.device != like.device or t.dim() != 1
-            or not t.is_contiguous() or (count is not None and t.shape[0] != count)):
-        raise ValueError(f"{name} must be a contiguous int32 tensor"
-                         f"{'' if count is None else f' of {count} elements'} on {like.device}")
-    return t.data_ptr()
+def _index(t, name, index, count):
+    try:
+        if t.dtype is _I32 and t.get_device() == index and t.shape == (count,) and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    raise ValueError(f"{name} must be a contiguous int32 tensor of {count} elements on x's device")
 
 
-def _sequences(x, offsets):
-    """(sequences, length, rows, offsets address) of ``x``; length 0 with offsets."""
-    dims = x.dim()
+def _sequences(shape, offsets, index):
+    """(sequences, length, rows, offsets address) of x; length 0 with offsets."""
     if offsets is not None:
-        if dims != 2:
+        if len(shape) != 2:
             raise ValueError("Packed sequences (offsets) require x of shape [rows, channels]")
-        address = _index(offsets, "offsets", x, None)
-        if offsets.shape[0] < 1:
+        count = offsets.shape[0] if isinstance(offsets, torch.Tensor) and offsets.dim() else 0
+        if count < 1:
             raise ValueError("offsets must hold n + 1 elements")
-        return offsets.shape[0] - 1, 0, x.shape[0], address
-    if dims == 2:
-        return x.shape[0], 1, x.shape[0], 0
-    if dims == 3:
-        if x.shape[1] < 1:
+        return count - 1, 0, shape[0], _index(offsets, "offsets", index, count)
+    if len(shape) == 2:
+        return shape[0], 1, shape[0], 0
+    if len(shape) == 3:
+        if shape[1] < 1:
             raise ValueError("Sequences without offsets must have at least one row")
-        return x.shape[0], x.shape[1], x.shape[0] * x.shape[1], 0
+        return shape[0], shape[1], shape[0] * shape[1], 0
     raise ValueError("x must have shape [rows, channels] or [n, length, channels]")
 
 
-def _states(state, codes, x, n, shape, dtype):
+def _states(state, codes, dtype, index, n, shape):
     """Addresses of a state pool and its codes, and its slots (0s for None)."""
     if state is None and codes is None:
         return 0, 0, 0
     if state is None or codes is None:
         raise ValueError("state and codes go together")
-    if (not isinstance(state, torch.Tensor) or state.dtype != dtype or state.device != x.device
-            or state.shape[1:] != shape or not state.is_contiguous()):
-        raise ValueError(f"state must be a contiguous {dtype} tensor of shape {['slots', *shape]} on {x.device}")
-    if state.shape[0] < n:
-        raise ValueError(f"{n} sequences need at least as many slots; state has {state.shape[0]}")
-    return state.data_ptr(), _index(codes, "codes", x, n), state.shape[0]
-
-
-def _status(status, x):
-    return 0 if status is None else _index(status, "status", x, 1)
-
-
-def _output(out, x):
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    try:
+        held = state.shape
+        good = state.dtype is dtype and state.get_device() == index and held[1:] == shape and state.is_contiguous()
+    except AttributeError:
+        good = False
+    if not good:
+        raise ValueError(f"state must be a contiguous {dtype} tensor of shape {['slots', *shape]} on x's device")
+    if held[0] < n:
+        raise ValueError(f"{n} sequences need at least as many slots; state has {held[0]}")
+    return state.data_ptr(), _index(codes, "codes", index, n), held[0]
 
 
 def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=None, codes=None, status=None, out=None):
@@ -185,39 +187,46 @@ def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=No
     sequence's first come from ``state`` ``[slots, 2, taps - 1, channels]`` (x's
     type, oldest first; ``conv_state`` makes one) or are zero.
     """
-    kind, device = _main(x)
+    kind, index = _main(x)
     _graph_free(x, weight, bias)
-    n, length, rows, offsets_at = _sequences(x, offsets)
-    channels = x.shape[-1]
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
+    shape, dtype = x.shape, x.dtype
+    n, length, rows, offsets_at = _sequences(shape, offsets, index)
+    channels = shape[-1]
+    taps = weight.shape[1] if isinstance(weight, torch.Tensor) and weight.dim() == 2 else 0
+    if not 2 <= taps <= 8:
         raise ValueError("weight must have shape [channels, taps] with 2 to 8 taps")
-    if activation not in (None, "silu"):
+    if activation is not None and activation != "silu":
         raise ValueError("activation must be None or 'silu'")
-    taps = weight.shape[1]
-    weight_at = _vector(weight, "weight", x, (channels, taps))
-    bias_at = _vector(bias, "bias", x, (channels,))
-    x_at, x_stride = _array(x, "x", x, x.shape)
-    pool_at, codes_at, slots = _states(state, codes, x, n, (2, taps - 1, channels), x.dtype)
-    status_at = _status(status, x)
-    lib = _library(device)
-    out = _output(out, x)
-    y_at, y_stride = _array(out, "out", x, x.shape)
+    weight_at = _vector(weight, "weight", index, (channels, taps))
+    bias_at = _vector(bias, "bias", index, (channels,))
+    x_at, x_stride = _array(x, "x", dtype, index, shape)
+    pool_at, codes_at, slots = _states(state, codes, dtype, index, n, (2, taps - 1, channels))
+    status_at = _index(status, "status", index, 1) if status is not None else 0
+    lib = _library(index)
+    if out is None:
+        out = torch.empty_like(x)
+    y_at, y_stride = _array(out, "out", dtype, index, shape)
     if n:
         _call(lib, lib.fav_causal_conv,
-              ConvArgs(x_at, y_at, x_stride, y_stride, weight_at, bias_at, pool_at, codes_at, offsets_at, status_at,
-                       kind, channels, taps, _ACTIVATIONS[activation], n, length, rows, slots), device)
+              CONV_ARGS(x_at, y_at, x_stride, y_stride, weight_at, bias_at, pool_at, codes_at, offsets_at, status_at,
+                        kind, channels, taps, _ACTIVATIONS[activation], n, length, rows, slots), index)
     return out
 
 
-def _maps(t, name, x, lead, groups, states):
+def _maps(t, name, dtype, index, lead, groups, states):
     """Address, row stride and group stride of an input or output map."""
-    if (not isinstance(t, torch.Tensor) or t.dtype != x.dtype or t.device != x.device
-            or t.shape[:-2] != lead or t.shape[-2:] != (groups, states)):
-        raise ValueError(f"{name} must be a {x.dtype} tensor of shape {[*lead, groups, states]} on {x.device}")
+    shape = (*lead, groups, states)
+    try:
+        good = t.dtype is dtype and t.get_device() == index and t.shape == shape
+    except AttributeError:
+        good = False
+    if not good:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)} on x's device")
     strides = t.stride()
     if strides[-1] != 1 and states != 1:
         raise ValueError(f"{name} must have adjacent states (stride 1)")
-    return t.data_ptr(), _row_stride(name, t.shape, strides, None), strides[-2] if groups > 1 else 0
+    return (t.data_ptr(), strides[0] if len(lead) == 1 else _row_stride(name, shape, strides),
+            strides[-2] if groups > 1 else 0)
 
 
 def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=True, offsets=None, state=None,
@@ -235,41 +244,44 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
     is ``[N, channels]`` and ``d`` and ``dt_bias`` are ``[channels]``. N is 1 to
     128. ``state`` is ``[slots, 2, N, channels]`` fp32 (``scan_state``).
     """
-    kind, device = _main(x)
+    kind, index = _main(x)
     _graph_free(x, dt, a, b, c, d, z, dt_bias)
-    n, length, rows, offsets_at = _sequences(x, offsets)
-    shape = x.shape
+    shape, dtype = x.shape, x.dtype
+    n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
-    if not isinstance(a, torch.Tensor) or a.dim() != 2 or not 1 <= a.shape[0] <= 128:
+    states = a.shape[0] if isinstance(a, torch.Tensor) and a.dim() == 2 else 0
+    if not 1 <= states <= 128:
         raise ValueError("a must have shape [states, channels] with 1 to 128 states")
-    states = a.shape[0]
-    if not isinstance(b, torch.Tensor) or b.dim() != x.dim() + 1 or b.shape[-2] < 1 or channels % b.shape[-2]:
+    groups = b.shape[-2] if isinstance(b, torch.Tensor) and b.dim() == len(shape) + 1 else 0
+    if groups < 1 or channels % groups:
         raise ValueError("b must have shape [..., groups, states] with groups that divide the channels")
-    groups = b.shape[-2]
-    x_at, x_stride = _array(x, "x", x, shape)
-    dt_at, dt_stride = _array(dt, "dt", x, shape)
-    z_at, z_stride = _array(z, "z", x, shape) if z is not None else (0, 0)
-    b_at, b_stride, b_group = _maps(b, "b", x, shape[:-1], groups, states)
-    c_at, c_stride, c_group = _maps(c, "c", x, shape[:-1], groups, states)
-    a_at = _vector(a, "a", x, (states, channels))
-    d_at = _vector(d, "d", x, (channels,))
-    bias_at = _vector(dt_bias, "dt_bias", x, (channels,))
-    pool_at, codes_at, slots = _states(state, codes, x, n, (2, states, channels), _F32)
-    status_at = _status(status, x)
-    lib = _library(device)
-    out = _output(out, x)
-    y_at, y_stride = _array(out, "out", x, shape)
+    x_at, x_stride = _array(x, "x", dtype, index, shape)
+    dt_at, dt_stride = _array(dt, "dt", dtype, index, shape)
+    z_at, z_stride = _array(z, "z", dtype, index, shape) if z is not None else (0, 0)
+    lead = shape[:-1]
+    b_at, b_stride, b_group = _maps(b, "b", dtype, index, lead, groups, states)
+    c_at, c_stride, c_group = _maps(c, "c", dtype, index, lead, groups, states)
+    a_at = _vector(a, "a", index, (states, channels))
+    d_at = _vector(d, "d", index, (channels,))
+    bias_at = _vector(dt_bias, "dt_bias", index, (channels,))
+    pool_at, codes_at, slots = _states(state, codes, _F32, index, n, (2, states, channels))
+    status_at = _index(status, "status", index, 1) if status is not None else 0
+    lib = _library(index)
+    if out is None:
+        out = torch.empty_like(x)
+    y_at, y_stride = _array(out, "out", dtype, index, shape)
     if not n:
         return out
-    args = ScanArgs(x_at, dt_at, z_at, b_at, c_at, y_at, x_stride, dt_stride, z_stride, b_stride, b_group, c_stride,
-                    c_group, y_stride, a_at, d_at, bias_at, pool_at, codes_at, offsets_at, status_at, 0, 0, kind,
-                    channels, states, groups, bool(softplus), n, length, rows, slots)
+    fixed = (x_at, dt_at, z_at, b_at, c_at, y_at, x_stride, dt_stride, z_stride, b_stride, b_group, c_stride, c_group,
+             y_stride, a_at, d_at, bias_at, pool_at, codes_at, offsets_at, status_at)
+    sizes = (kind, channels, states, groups, bool(softplus), n, length, rows, slots)
+    args = SCAN_ARGS(*fixed, 0, 0, *sizes)
     if length != 1:
-        need = lib.fav_selective_scan_workspace_bytes(ct.byref(args))
+        need = lib.fav_selective_scan_workspace_bytes(args)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            args.workspace, args.workspace_bytes = workspace.data_ptr(), need
-    _call(lib, lib.fav_selective_scan, args, device)
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+            args = SCAN_ARGS(*fixed, workspace.data_ptr(), need, *sizes)
+    _call(lib, lib.fav_selective_scan, args, index)
     return out
 
 
@@ -284,10 +296,11 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     ``activation`` is None, ``"silu"`` or ``"snake"``, the decoder's
     ``v + reciprocal * sin(alpha * v)**2`` with ``[channels]`` coefficients.
     """
-    kind, device = _main(x)
+    kind, index = _main(x)
     _graph_free(x, weight, bias, alpha, reciprocal)
-    n, length, rows, offsets_at = _sequences(x, offsets)
-    channels = x.shape[-1]
+    shape, dtype = x.shape, x.dtype
+    n, length, rows, offsets_at = _sequences(shape, offsets, index)
+    channels = shape[-1]
     if type(groups) is not int or groups < 1 or channels % groups:
         raise ValueError("groups must be a positive int that divides the channels")
     if activation not in _ACTIVATIONS:
@@ -296,18 +309,19 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
         raise ValueError("alpha and reciprocal belong to activation='snake'")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    shape = (channels,)
-    coefficients = (_vector(weight, "weight", x, shape), _vector(bias, "bias", x, shape),
-                    _vector(alpha, "alpha", x, shape), _vector(reciprocal, "reciprocal", x, shape))
-    x_at, x_stride = _array(x, "x", x, x.shape)
-    status_at = _status(status, x)
-    lib = _library(device)
-    out = _output(out, x)
-    y_at, y_stride = _array(out, "out", x, x.shape)
+    per = (channels,)
+    coefficients = (_vector(weight, "weight", index, per), _vector(bias, "bias", index, per),
+                    _vector(alpha, "alpha", index, per), _vector(reciprocal, "reciprocal", index, per))
+    x_at, x_stride = _array(x, "x", dtype, index, shape)
+    status_at = _index(status, "status", index, 1) if status is not None else 0
+    lib = _library(index)
+    if out is None:
+        out = torch.empty_like(x)
+    y_at, y_stride = _array(out, "out", dtype, index, shape)
     if n:
         _call(lib, lib.fav_group_norm,
-              NormArgs(x_at, y_at, x_stride, y_stride, *coefficients, offsets_at, status_at, eps, kind, channels,
-                       groups, _ACTIVATIONS[activation], n, length, rows), device)
+              NORM_ARGS(x_at, y_at, x_stride, y_stride, *coefficients, offsets_at, status_at, eps, kind, channels,
+                        groups, _ACTIVATIONS[activation], n, length, rows), index)
     return out
 
 
@@ -320,31 +334,39 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
     (``quantize_int4`` makes both), ``x`` ``[rows, depth]``. ``group`` and the
     depth are multiples of 32.
     """
-    kind, device = _main(x)
+    kind, index = _main(x)
     _graph_free(x, scales, bias)
-    if x.dim() != 2:
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2:
         raise ValueError("x must have shape [rows, depth]")
-    rows, depth = x.shape
+    rows, depth = shape
     if type(group) is not int or group < 32 or group % 32 or depth < 32 or depth % 32:
         raise ValueError("group and the depth must be positive multiples of 32")
-    if (not isinstance(weight, torch.Tensor) or weight.dtype != torch.uint8 or weight.device != device
-            or weight.dim() != 2 or weight.shape[1] != depth // 2 or not weight.is_contiguous()):
-        raise ValueError(f"weight must be a contiguous uint8 tensor of shape ['out', {depth // 2}] on {device}")
-    if weight.data_ptr() % 16:
+    try:
+        packed = weight.shape
+        good = (weight.dtype is torch.uint8 and weight.get_device() == index and len(packed) == 2
+                and packed[1] == depth // 2 and weight.is_contiguous())
+    except AttributeError:
+        good = False
+    if not good:
+        raise ValueError(f"weight must be a contiguous uint8 tensor of shape ['out', {depth // 2}] on x's device")
+    weight_at = weight.data_ptr()
+    if weight_at % 16:
         raise ValueError("weight must be 16-byte aligned")
-    width = weight.shape[0]
     if scales is None:
         raise ValueError("scales are required")
-    scales_at = _vector(scales, "scales", x, (width, -(-depth // group)))
-    bias_at = _vector(bias, "bias", x, (width,))
-    x_at, x_stride = _array(x, "x", x, x.shape)
-    lib = _library(device)
-    out = torch.empty((rows, width), dtype=x.dtype, device=device) if out is None else out
-    y_at, y_stride = _array(out, "out", x, (rows, width))
+    width = packed[0]
+    scales_at = _vector(scales, "scales", index, (width, -(-depth // group)))
+    bias_at = _vector(bias, "bias", index, (width,))
+    x_at, x_stride = _array(x, "x", dtype, index, shape)
+    lib = _library(index)
+    if out is None:
+        out = x.new_empty((rows, width))
+    y_at, y_stride = _array(out, "out", dtype, index, (rows, width))
     if rows and width:
         _call(lib, lib.fav_project_int4,
-              Int4Args(x_at, y_at, x_stride, y_stride, weight.data_ptr(), scales_at, bias_at, kind, rows, depth, width,
-                       group), device)
+              INT4_ARGS(x_at, y_at, x_stride, y_stride, weight_at, scales_at, bias_at, kind, rows, depth, width, group),
+              index)
     return out
 
 
