@@ -1,8 +1,23 @@
-// Projection of a few rows by 4-bit weights with group scales:
+// Projection of the few rows of a step by 4-bit weights with group scales:
 //
 //   y[m, r] = bias[r] + sum_g scales[r, g] * sum_{k in g} x[m, k] * (q[r, k] - 8)
 //
-// Sums in fp32.
+// Bound by reading the weights once (out * depth / 2 bytes). The codes minus 8
+// are exact in fp16 and bf16, so the inner sums run on the tensor cores with
+// exact operands: mma.sync m16n8k16, 16 weight rows by 8 input rows, fp32
+// accumulation (an input row or two cannot fill a tcgen05 tile, and the codes
+// must pass the registers anyway to become operands). A block's sum is scaled
+// and joined in fp32. fp32 inputs are cut into three bf16 parts of 8 bits each
+// that add up to them exactly: three products, one accumulator.
+//
+// Layout. Weights stay as the caller has them, row after row. An MMA does not
+// care in which order it walks k as long as both operands agree, so a lane
+// takes W consecutive bytes (2 W values of k) of its two rows and the same
+// values of k of its input row; four lanes make a k block of 8 W values. W is
+// the widest of 16, 8 and 4 with blocks that a group's scale covers whole.
+// A CTA owns 16 R rows and all of k; its eight warps take every eighth k block,
+// with up to U blocks of weights on their way at once, and join through shared
+// memory in a fixed order.
 #include "fav_ops.cuh"
 
 namespace fav {
@@ -14,44 +29,247 @@ struct Int4Args {
   long long x_stride, y_stride;
   const uint8_t* weight;
   const float *scales, *bias;
-  int rows, depth, out, group;
+  int rows, depth, out, group, groups;
+  int wide;  // input rows start on 16-byte boundaries
 };
 
-constexpr int kInt4Threads = 128;
+constexpr int kInt4Warps = 8;
+constexpr int kInt4Threads = 32 * kInt4Warps;
 
+// The MMA's operand type for inputs of type T, and the parts of an input.
 template <typename T>
-__global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constant__ Int4Args a) {
-  grid_dependency_sync();
-  const long long warp = ((long long)blockIdx.x * kInt4Threads + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  const int m = (int)(warp / a.out), r = (int)(warp - (long long)m * a.out);
-  if (m >= a.rows) return;
-  const int groups = (a.depth + a.group - 1) / a.group;
-  const T* x = static_cast<const T*>(a.x) + m * a.x_stride;
-  const uint8_t* w = a.weight + (size_t)r * (a.depth / 2);
-  float sum = 0.f;
-  for (int k = 2 * lane; k < a.depth; k += 64) {
-    const int byte = w[k / 2];
-    const float s = a.scales[(size_t)r * groups + k / a.group];
-    sum = fmaf(s, to_f32(x[k]) * (float)((byte & 15) - 8) + to_f32(x[k + 1]) * (float)((byte >> 4) - 8), sum);
+struct Int4Type {
+  using M = T;
+  static constexpr int kParts = 1;
+};
+template <>
+struct Int4Type<float> {
+  using M = __nv_bfloat16;
+  static constexpr int kParts = 3;
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                          __nv_bfloat16) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Codes j and j + 4 of a word of eight, minus 8, as a pair of operands. The
+// code is put into the mantissa of 1024 (fp16) or 128 (bf16); taking 1032 or
+// 136 away is exact.
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, int j, __half) {
+  const uint32_t v = ((word >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __floats2half2_rn(1032.f, 1032.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t code_pair(uint32_t word, int j, __nv_bfloat16) {
+  const uint32_t v = ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(136.f, 136.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Eight inputs as the four pairs (0,4), (1,5), (2,6), (3,7) of each part.
+template <typename T>
+__device__ __forceinline__ void input_pairs(const T* p, bool wide, uint32_t (&b)[1][4]) {
+  uint32_t w[4];
+  if (wide) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0)
-    static_cast<T*>(a.y)[m * a.y_stride + r] = from_f32<T>(a.bias ? sum + __ldg(a.bias + r) : sum);
+  for (int i = 0; i < 2; ++i) {
+    b[0][2 * i] = __byte_perm(w[i], w[i + 2], 0x5410);
+    b[0][2 * i + 1] = __byte_perm(w[i], w[i + 2], 0x7632);
+  }
+}
+__device__ __forceinline__ void input_pairs(const float* p, bool wide, uint32_t (&b)[3][4]) {
+  float v[8];
+  if (wide) {
+    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[i];
+  }
+  uint32_t part[3][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // Truncation, so that the largest values do not round to infinity; what is
+    // not finite stays in the first part alone (with a NaN's leading bit).
+    const uint32_t bits = __float_as_uint(v[i]);
+    const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+    const bool nan = !finite && (bits & 0x007fffffu);
+    part[0][i] = (bits & 0xffff0000u) | (nan ? 0x00400000u : 0u);
+    const float mid = v[i] - __uint_as_float(bits & 0xffff0000u);
+    part[1][i] = finite ? __float_as_uint(mid) & 0xffff0000u : 0u;
+    part[2][i] = finite ? __float_as_uint(mid - __uint_as_float(part[1][i])) : 0u;
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[q][i] = __byte_perm(part[q][i], part[q][i + 4], 0x7632);
+}
+
+// W consecutive weight bytes of one lane and row.
+template <int W>
+struct Codes {
+  uint32_t w[W / 4];
+};
+template <int W>
+__device__ __forceinline__ Codes<W> load_codes(const uint8_t* p) {
+  Codes<W> c;
+  if constexpr (W == 16) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
+  } else if constexpr (W == 8) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    c.w[0] = v.x, c.w[1] = v.y;
+  } else {
+    c.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+  return c;
+}
+
+// R: tiles of 16 weight rows a warp; C: tiles of 8 input rows.
+template <typename T, int W, int R, int C>
+__global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constant__ Int4Args a) {
+  using M = typename Int4Type<T>::M;
+  constexpr int P = Int4Type<T>::kParts, KB = 8 * W, U = 64 / (W * R);
+  constexpr int kOut = 16 * R, kIn = 8 * C;
+  __shared__ float s_sum[kInt4Warps][kIn][kOut + 1];
+  grid_dependency_sync();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = blockIdx.x * kOut, m0 = blockIdx.y * kIn;
+  const int blocks = (a.depth + KB - 1) / KB;
+  const size_t pitch = a.depth / 2;
+  const uint8_t* wrow[R][2];
+  const float* srow[R][2];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = min(r0 + 16 * r + 8 * h + g, a.out - 1);  // rows behind the last repeat it, unused
+      wrow[r][h] = a.weight + row * pitch + t * W;
+      srow[r][h] = a.scales + (size_t)row * a.groups;
+    }
+  float sum[R][C][4] = {};
+  for (int b0 = warp; b0 < blocks; b0 += kInt4Warps * U) {
+    Codes<W> code[U][R][2];
+    float scale[U][R][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int blk = b0 + u * kInt4Warps;
+      const bool in = blk * KB + t * 2 * W < a.depth;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          code[u][r][h] = in ? load_codes<W>(wrow[r][h] + (size_t)blk * (KB / 2)) : Codes<W>{};
+          scale[u][r][h] = blk < blocks ? __ldg(srow[r][h] + blk * KB / a.group) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int blk = b0 + u * kInt4Warps;
+      if (blk >= blocks) break;
+      const int k = blk * KB + t * 2 * W;
+      float part[R][C][4] = {};
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        uint32_t op[R][2][4];  // two MMAs of a word of eight codes
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            op[r][j / 2][2 * (j % 2)] = code_pair(code[u][r][0].w[i], j, M{});
+            op[r][j / 2][2 * (j % 2) + 1] = code_pair(code[u][r][1].w[i], j, M{});
+          }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int m = m0 + 8 * c + g;
+          uint32_t in[P][4] = {};
+          if (m < a.rows && k + 8 * i < a.depth)
+            input_pairs(static_cast<const T*>(a.x) + m * a.x_stride + k + 8 * i, a.wide != 0, in);
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int q = P - 1; q >= 0; --q) {
+              mma_16816(part[r][c], op[r][0], in[q][0], in[q][1], M{});
+              mma_16816(part[r][c], op[r][1], in[q][2], in[q][3], M{});
+            }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[r][c][e] = fmaf(scale[u][r][e / 2], part[r][c][e], sum[r][c][e]);
+    }
+  }
+  // Accumulators 0, 1: weight row g, input rows 2 t and 2 t + 1; 2, 3: row g + 8.
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s_sum[warp][8 * c + 2 * t + e % 2][16 * r + 8 * (e / 2) + g] = sum[r][c][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kIn * kOut; i += kInt4Threads) {
+    const int c = i / kOut, r = i % kOut, m = m0 + c, row = r0 + r;
+    if (m >= a.rows || row >= a.out) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kInt4Warps; ++w) v += s_sum[w][c][r];
+    static_cast<T*>(a.y)[m * a.y_stride + row] = from_f32<T>(a.bias ? v + __ldg(a.bias + row) : v);
+  }
+}
+
+template <typename T, int W, int R, int C>
+cudaError_t launch_tile(const Int4Args& a, cudaStream_t stream) {
+  const long long across = ((long long)a.rows + 8 * C - 1) / (8 * C);
+  if (across > 65535) return cudaErrorInvalidValue;
+  return launch_op(int4_kernel<T, W, R, C>, dim3((a.out + 16 * R - 1) / (16 * R), (unsigned)across), kInt4Threads, 0,
+                   stream, a);
+}
+
+template <typename T, int W>
+cudaError_t launch_width(const Int4Args& a, cudaStream_t stream) {
+  // 32 weight rows a CTA where that still gives every SM one: the inputs are
+  // then read and arranged half as often. Up to 32 input rows share a pass
+  // over the weights.
+  if (a.rows <= 8) return a.out >= 148 * 32 ? launch_tile<T, W, 2, 1>(a, stream) : launch_tile<T, W, 1, 1>(a, stream);
+  if (a.rows <= 16) return launch_tile<T, W, 1, 2>(a, stream);
+  return launch_tile<T, W, 1, 4>(a, stream);
+}
+
+template <typename T>
+cudaError_t launch_group(const Int4Args& a, cudaStream_t stream) {
+  if (a.group % 128 == 0) return launch_width<T, 16>(a, stream);
+  if (a.group % 64 == 0) return launch_width<T, 8>(a, stream);
+  return launch_width<T, 4>(a, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_project_int4(const fav_int4_args& c, cudaStream_t stream) {
-  Int4Args a{c.x, c.y, c.x_stride, c.y_stride, c.weight, c.scales, c.bias, c.rows, c.depth, c.out, c.group};
-  const long long blocks = ((long long)c.rows * c.out + kInt4Threads / 32 - 1) / (kInt4Threads / 32);
-  if (blocks == 0) return cudaSuccess;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (c.type == FAV_TYPE_F32) return launch_op(int4_kernel<float>, (unsigned)blocks, kInt4Threads, 0, stream, a);
-  if (c.type == FAV_TYPE_BF16)
-    return launch_op(int4_kernel<__nv_bfloat16>, (unsigned)blocks, kInt4Threads, 0, stream, a);
-  return launch_op(int4_kernel<__half>, (unsigned)blocks, kInt4Threads, 0, stream, a);
+  Int4Args a{c.x, c.y, c.x_stride, c.y_stride, c.weight, c.scales, c.bias, c.rows, c.depth, c.out, c.group,
+             (c.depth + c.group - 1) / c.group, 0};
+  const int elem = elem_bytes(c.type);
+  a.wide = aligned_for(c.x, c.x_stride, elem, 16 / elem);
+  if (c.type == FAV_TYPE_F32) return launch_group<float>(a, stream);
+  if (c.type == FAV_TYPE_BF16) return launch_group<__nv_bfloat16>(a, stream);
+  return launch_group<__half>(a, stream);
 }
 
 }  // namespace fav
