@@ -42,9 +42,35 @@ template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
 }
+// The same of memory that no thread writes during the kernel.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_const(const T* p) {
+  constexpr int B = sizeof(T) * V;
+  Pack<T, V> r;
+  if constexpr (B == 16)
+    *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
+  else if constexpr (B == 8)
+    *reinterpret_cast<uint2*>(&r) = __ldg(reinterpret_cast<const uint2*>(p));
+  else if constexpr (B == 4)
+    *reinterpret_cast<uint32_t*>(&r) = __ldg(reinterpret_cast<const uint32_t*>(p));
+  else
+    *reinterpret_cast<uint16_t*>(&r) = __ldg(reinterpret_cast<const uint16_t*>(p));
+  return r;
+}
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
   *reinterpret_cast<Pack<T, V>*>(p) = v;
+}
+
+// Elements 2 i and 2 i + 1 of a pack in fp32, and back. V = 1: element 0 twice.
+template <typename T, int V>
+__device__ __forceinline__ float2 pair_of(const Pack<T, V>& p, int i) {
+  return make_float2(to_f32(p.v[V > 1 ? 2 * i : 0]), to_f32(p.v[V > 1 ? 2 * i + 1 : 0]));
+}
+template <typename T, int V>
+__device__ __forceinline__ void put_pair(Pack<T, V>& p, int i, float2 v) {
+  p.v[V > 1 ? 2 * i : 0] = from_f32<T>(v.x);
+  if constexpr (V > 1) p.v[2 * i + 1] = from_f32<T>(v.y);
 }
 
 __device__ __forceinline__ float ex2_approx(float v) {
@@ -54,10 +80,30 @@ __device__ __forceinline__ float ex2_approx(float v) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// v / (1 + e^-v); at -inf the quotient of -inf by +inf is replaced by its limit.
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// v / (1 + e^-v) by the hardware's 2^x and 1/x (2 and 1 units in the last
+// place). Below -100, where e^-v overflows, v stands at -100: the result is
+// then 0, its limit, at -inf too. A NaN stays one.
 __device__ __forceinline__ float silu(float v) {
-  const float y = __fdividef(v, 1.f + __expf(-v));
-  return v < -87.f ? 0.f : y;
+  v = max_nan(v, -100.f);
+  return v * rcp_approx(1.f + ex2_approx(-kLog2e * v));
+}
+// The same of two, the multiplies and the sum packed.
+__device__ __forceinline__ float2 silu2(float2 v) {
+  v = make_float2(max_nan(v.x, -100.f), max_nan(v.y, -100.f));
+  const float2 p = f2mul(v, make_float2(-kLog2e, -kLog2e));
+  const float2 s = f2add(make_float2(ex2_approx(p.x), ex2_approx(p.y)), make_float2(1.f, 1.f));
+  return f2mul(v, make_float2(rcp_approx(s.x), rcp_approx(s.y)));
 }
 
 // --------------------------------------------------------------- sequences

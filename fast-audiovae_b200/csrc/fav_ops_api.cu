@@ -13,7 +13,7 @@ cudaError_t launch_project_int4(const fav_int4_args&, cudaStream_t);
 
 namespace {
 
-constexpr long long kMaxRows = 0x7ffffff0;
+constexpr long long kMaxRows = 0x7fff0000;
 constexpr int kMaxChannels = 1 << 20;
 
 // Rows, channels and sequences that index arithmetic and grids can hold.
