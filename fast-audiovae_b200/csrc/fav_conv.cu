@@ -142,23 +142,6 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const __grid_co
   }
 }
 
-// One row of a thread's channels from global memory into its own place in
-// shared memory, asynchronously; without an asynchronous copy of that size
-// (2 bytes) at once.
-template <typename T, int V>
-__device__ __forceinline__ void copy_row(Pack<T, V>* to, const T* from) {
-  if constexpr (sizeof(T) * V >= 4)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(sizeof(T) * V)
-                 : "memory");
-  else
-    *to = load_const<T, V>(from);
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 template <typename T, int V, int K, bool ACT>
 __global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(const __grid_constant__ ConvArgs a) {
   constexpr int H = K - 1, U = 4, D = kConvDepth;
@@ -197,7 +180,7 @@ __global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(cons
   T* py = static_cast<T*>(a.y) + c + r * a.y_stride;
 #pragma unroll
   for (int u = 0; u < D; ++u) {
-    if (r + u < last) copy_row<T, V>(ring + u * kConvThreads, px);
+    if (r + u < last) copy_pack<T, V>(ring + u * kConvThreads, px);
     copy_commit();
     px += a.x_stride;
   }
@@ -238,7 +221,7 @@ __global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(cons
       for (int u = 0; u < U; ++u) win[H + u] = widen(ring[(at + u) * kConvThreads]);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (r + D + u < last) copy_row<T, V>(ring + (at + u) * kConvThreads, px);
+        if (r + D + u < last) copy_pack<T, V>(ring + (at + u) * kConvThreads, px);
         copy_commit();
         px += a.x_stride;
       }
@@ -253,7 +236,7 @@ __global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(cons
     } else {
       copy_wait<D - 1>();
       win[H] = widen(ring[at * kConvThreads]);
-      if (r + D < last) copy_row<T, V>(ring + at * kConvThreads, px);
+      if (r + D < last) copy_pack<T, V>(ring + at * kConvThreads, px);
       copy_commit();
       px += a.x_stride;
       if (live) store_pack<T, V>(py, narrow<T, V>(th.row(win)));

@@ -40,26 +40,27 @@ struct NormArgs {
 };
 
 // sin(v)^2 has period pi: v - k pi lies within pi / 2 of zero, where the Taylor
-// series of the sine to the 13th power is exact to 1e-9. pi in two parts
+// series of the sine to the 11th power is within 6e-8. pi in two parts
 // (8 + 24 bits) keeps the difference exact to fp32 for |v| up to 2^14.
+__device__ __forceinline__ float2 both(float c) { return make_float2(c, c); }
 __device__ __forceinline__ float2 sin_squared2(float2 v) {
-  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: rounds to an integer
-  const float2 t = f2fma(v, make_float2(0.318309886f, 0.318309886f), magic);
-  const float2 k = f2add(t, make_float2(-12582912.f, -12582912.f));
-  float2 r = f2fma(k, make_float2(-3.140625f, -3.140625f), v);
-  r = f2fma(k, make_float2(-9.6765358979e-4f, -9.6765358979e-4f), r);
+  const float2 t = f2fma(v, both(0.318309886f), both(12582912.f));  // 1.5 * 2^23: rounds to an integer
+  const float2 k = f2add(t, both(-12582912.f));
+  float2 r = f2fma(k, both(-3.140625f), v);
+  r = f2fma(k, both(-9.6765358979e-4f), r);
   const float2 z = f2mul(r, r);
-  float2 p = make_float2(1.6059044e-10f, 1.6059044e-10f);
-  p = f2fma(p, z, make_float2(-2.5052108e-8f, -2.5052108e-8f));
-  p = f2fma(p, z, make_float2(2.7557319e-6f, 2.7557319e-6f));
-  p = f2fma(p, z, make_float2(-1.9841270e-4f, -1.9841270e-4f));
-  p = f2fma(p, z, make_float2(8.3333333e-3f, 8.3333333e-3f));
-  p = f2fma(p, z, make_float2(-1.6666667e-1f, -1.6666667e-1f));
+  float2 p = both(-2.5052108e-8f);
+  p = f2fma(p, z, both(2.7557319e-6f));
+  p = f2fma(p, z, both(-1.9841270e-4f));
+  p = f2fma(p, z, both(8.3333333e-3f));
+  p = f2fma(p, z, both(-1.6666667e-1f));
   const float2 s = f2fma(f2mul(r, z), p, r);
-  float2 q = f2mul(s, s);
-  if (!(fabsf(v.x) < 16384.f)) { const float e = sinf(v.x); q.x = e * e; }
-  if (!(fabsf(v.y) < 16384.f)) { const float e = sinf(v.y); q.y = e * e; }
-  return q;
+  return f2mul(s, s);
+}
+constexpr float kSineRange = 16384.f;
+__device__ __noinline__ float sin_squared_far(float v) {
+  const float s = sinf(v);
+  return s * s;
 }
 
 // The coefficients of V neighbouring channels, and their outputs.
@@ -92,41 +93,69 @@ struct NormChannels {
       pairs(re, a.recip, c, 0.f, a.wide);
     }
   }
-  template <typename T>
-  __device__ __forceinline__ Pack<T, V> apply(const NormArgs& a, const Pack<T, V>& x, float mean, float rstd) const {
-    Pack<T, V> out;
+  // After load(): w times rstd, so that a value takes one multiply.
+  __device__ __forceinline__ void scale(float rstd) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      float2 v = f2mul(f2add(pair_of(x, i), make_float2(-mean, -mean)), make_float2(rstd, rstd));
-      v = f2fma(v, w[i], b[i]);
-      if (a.activation == FAV_ACTIVATION_SILU)
-        v = silu2(v);
-      else if (a.activation == FAV_ACTIVATION_SNAKE)
-        v = f2fma(re[i], sin_squared2(f2mul(al[i], v)), v);
-      put_pair(out, i, v);
+    for (int i = 0; i < P; ++i) w[i] = f2mul(w[i], make_float2(rstd, rstd));
+  }
+  template <typename T>
+  __device__ __forceinline__ Pack<T, V> apply(int activation, const Pack<T, V>& x, float mean) const {
+    Pack<T, V> out;
+    float2 v[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = f2fma(f2add(pair_of(x, i), make_float2(-mean, -mean)), w[i], b[i]);
+    if (activation == FAV_ACTIVATION_SILU) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = silu2(v[i]);
+    } else if (activation == FAV_ACTIVATION_SNAKE) {
+      float2 u[P], q[P];
+      float far = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        u[i] = f2mul(al[i], v[i]);
+        far = fmaxf(far, fmaxf(fabsf(u[i].x), fabsf(u[i].y)));
+        q[i] = sin_squared2(u[i]);
+      }
+      if (far >= kSineRange) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          if (!(fabsf(u[i].x) < kSineRange)) q[i].x = sin_squared_far(u[i].x);
+          if (!(fabsf(u[i].y) < kSineRange)) q[i].y = sin_squared_far(u[i].y);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = f2fma(re[i], q[i], v[i]);
     }
+#pragma unroll
+    for (int i = 0; i < P; ++i) put_pair(out, i, v[i]);
     return out;
   }
 };
 
+// Sums over a pack's elements, the even and the odd ones apart (V = 1: the
+// element alone).
 template <typename T, int V>
-__device__ __forceinline__ float sum_of(const Pack<T, V>& x) {
-  float s = 0.f;
+__device__ __forceinline__ float2 add_values(const Pack<T, V>& x, float2 sum) {
+  if constexpr (V == 1) return make_float2(sum.x + to_f32(x.v[0]), 0.f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) s += to_f32(x.v[i]);
-  return s;
+  for (int i = 0; i < V / 2; ++i) sum = f2add(sum, pair_of(x, i));
+  return sum;
 }
 template <typename T, int V>
-__device__ __forceinline__ float squares_about(const Pack<T, V>& x, float mean, float sum) {
+__device__ __forceinline__ float2 add_squares(const Pack<T, V>& x, float mean, float2 sum) {
+  if constexpr (V == 1) {
+    const float d = to_f32(x.v[0]) - mean;
+    return make_float2(fmaf(d, d, sum.x), 0.f);
+  }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float d = to_f32(x.v[i]) - mean;
-    sum = fmaf(d, d, sum);
+  for (int i = 0; i < V / 2; ++i) {
+    const float2 d = f2add(pair_of(x, i), make_float2(-mean, -mean));
+    sum = f2fma(d, d, sum);
   }
   return sum;
 }
 
-constexpr int kNormThreads = 256;
+constexpr int kRowThreads = 256;  // single rows
 
 // ------------------------------------------------------------- single rows
 // `group_threads` threads (a power of two) hold a (row, group)'s values, NV
@@ -146,10 +175,10 @@ __device__ __forceinline__ float group_sum(float v, int threads, float* part) {
 }
 
 template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kNormThreads) norm_rows_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float part[kNormThreads / 32];
+__global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[kRowThreads / 32];
   grid_dependency_sync();
-  const int threads = a.group_threads, per_block = kNormThreads / threads;
+  const int threads = a.group_threads, per_block = kRowThreads / threads;
   const long long item = (long long)blockIdx.x * per_block + threadIdx.x / threads;
   const bool live = item < (long long)a.seq.rows * a.groups;
   const long long row = live ? item / a.groups : 0;
@@ -160,47 +189,64 @@ __global__ void __launch_bounds__(kNormThreads) norm_rows_kernel(const __grid_co
   const float inv = 1.f / (float)a.width;
   if constexpr (NV > 0) {
     Pack<T, V> xv[NV];
-    float sum = 0.f;
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (t + k * threads < vecs) {
         xv[k] = load_const<T, V>(x + (t + k * threads) * V);
-        sum += sum_of(xv[k]);
+        sum = add_values(xv[k], sum);
       }
-    const float mean = group_sum(sum, threads, part) * inv;
-    sum = 0.f;
+    const float mean = group_sum(sum.x + sum.y, threads, part) * inv;
+    sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (t + k * threads < vecs) sum = squares_about(xv[k], mean, sum);
-    const float rstd = rsqrtf(group_sum(sum, threads, part) * inv + a.eps);
+      if (t + k * threads < vecs) sum = add_squares(xv[k], mean, sum);
+    const float rstd = rsqrtf(group_sum(sum.x + sum.y, threads, part) * inv + a.eps);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (t + k * threads) * V;
       if (!live || t + k * threads >= vecs) continue;
       NormChannels<V> ch;
       ch.load(a, c0 + c);
-      store_pack<T, V>(y + c, ch.apply(a, xv[k], mean, rstd));
+      ch.scale(rstd);
+      store_pack<T, V>(y + c, ch.apply(a.activation, xv[k], mean));
     }
   } else {
-    float sum = 0.f;
-    for (int k = t; k < vecs; k += threads) sum += sum_of(load_const<T, V>(x + (size_t)k * V));
-    const float mean = group_sum(sum, threads, part) * inv;
-    sum = 0.f;
-    for (int k = t; k < vecs; k += threads) sum = squares_about(load_const<T, V>(x + (size_t)k * V), mean, sum);
-    const float rstd = rsqrtf(group_sum(sum, threads, part) * inv + a.eps);
+    float2 sum = make_float2(0.f, 0.f);
+    for (int k = t; k < vecs; k += threads) sum = add_values(load_const<T, V>(x + (size_t)k * V), sum);
+    const float mean = group_sum(sum.x + sum.y, threads, part) * inv;
+    sum = make_float2(0.f, 0.f);
+    for (int k = t; k < vecs; k += threads) sum = add_squares(load_const<T, V>(x + (size_t)k * V), mean, sum);
+    const float rstd = rsqrtf(group_sum(sum.x + sum.y, threads, part) * inv + a.eps);
     for (int k = t; live && k < vecs; k += threads) {
       NormChannels<V> ch;
       ch.load(a, c0 + k * V);
-      store_pack<T, V>(y + (size_t)k * V, ch.apply(a, load_const<T, V>(x + (size_t)k * V), mean, rstd));
+      ch.scale(rstd);
+      store_pack<T, V>(y + (size_t)k * V, ch.apply(a.activation, load_const<T, V>(x + (size_t)k * V), mean));
     }
   }
 }
 
+constexpr int kThreads = 128, kWideThreads = 512;  // of a CTA: its share of the rows small or large
+constexpr int kMaxCtas = 16;  // of a cluster (above 8 where the device can place them)
+
 // --------------------------------------------------------------- sequences
 // A CTA's share of one (sequence, block of groups): rows [first, first + rows)
 // by vecs vectors, walked by threads in the order of e = row * vecs + vector. A
-// block of several groups has at most kNormThreads vectors, and only whole
+// block of several groups has at most NT vectors, and only whole
 // rows of threads walk it: a thread then keeps to one vector, hence one group.
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, float* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) v += part[i];
+  return v;
+}
+
 struct Stats {
   float count, mean, squares;
 };
@@ -212,10 +258,13 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
   return {n, fmaf(d, f, a.mean), a.squares + b.squares + d * d * a.count * f};
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads) norm_kernel(const __grid_constant__ NormArgs a) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+template <typename T, int V, int NT>
+__global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(const __grid_constant__ NormArgs a) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  __shared__ float s_sum[kNormThreads], s_square[kNormThreads];
+  __shared__ float s_sum[NT], s_square[NT];
   using P = Pack<T, V>;
   P* kept = reinterpret_cast<P*>(s_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -233,76 +282,112 @@ __global__ void __launch_bounds__(kNormThreads) norm_kernel(const __grid_constan
   const int c0 = g0 * a.width, vecs = groups * a.width / V, group_vecs = a.width / V;
   const T* x = static_cast<const T*>(a.x) + (sp.begin + before) * a.x_stride + c0;
   T* y = static_cast<T*>(a.y) + (sp.begin + before) * a.y_stride + c0;
-  const int step = vecs <= kNormThreads ? kNormThreads / vecs * vecs : kNormThreads;
+  const int step = vecs <= NT ? NT / vecs * vecs : NT;
   const bool walks = threadIdx.x < step;
   // Row and vector of a thread, and its steps from one to the next.
   const int r0 = threadIdx.x / vecs, v0 = threadIdx.x - r0 * vecs, dr = step / vecs, dv = step - dr * vecs;
-  constexpr int U = 8;  // vectors on their way at once
-
-  float sum = 0.f, count = 0.f;
-  for (int r = r0, v = v0; walks && r < rows;) {
-    P in[U];
-    int n = 0;
-    int rr = r, vv = v;
+  // Vectors of this thread, the kept ones first.
+  const int vectors = walks && rows > r0 ? (int)(((long long)rows * vecs - threadIdx.x - 1) / step) + 1 : 0;
+  const int held = min(rows, a.keep_rows);
+  const int kept_vectors = walks && held > r0 ? (held * vecs - (int)threadIdx.x - 1) / step + 1 : 0;
+  float2 sums = make_float2(0.f, 0.f);
+  if (dv == 0) {
+    const T* p = x + r0 * a.x_stride + v0 * V;
+    P* to = kept + threadIdx.x;
+    const long long hop = dr * a.x_stride;
+    if constexpr (V == 8) {
+      // 16 vectors are on their way to their places, four of them summed at a
+      // time: the sums of 8 take long enough to hide loads behind (64 clips of
+      // 750 x 512 bf16: 29 us, all rows first 36).
+      int issued = 0;
+      const auto issue = [&] {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (rr < rows) {
-        in[u] = load_const<T, V>(x + rr * a.x_stride + vv * V);
-        n = u + 1;
+        for (int u = 0; u < 4; ++u, ++issued, p += hop)
+          if (issued < kept_vectors) copy_pack<T, V>(to + issued * step, p);
+        copy_commit();
+      };
+      issue();
+      issue();
+      issue();
+      for (int k = 0; k < kept_vectors; k += 4) {
+        issue();
+        copy_wait<3>();
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (k + u < kept_vectors) sums = add_values(to[(k + u) * step], sums);
       }
-      rr += dr, vv += dv;
-      if (vv >= vecs) ++rr, vv -= vecs;
+    } else {
+      // All of the kept rows are on their way at once, then summed (fp32 44 us, as
+      // above 49).
+#pragma unroll 4
+      for (int k = 0; k < kept_vectors; ++k, p += hop) copy_pack<T, V>(to + k * step, p);
+      copy_commit();
+      copy_wait<0>();
+#pragma unroll 4
+      for (int k = 0; k < kept_vectors; ++k) sums = add_values(to[k * step], sums);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u < n) {
-        sum += sum_of(in[u]);
-        count += V;
-        if (r < a.keep_rows) kept[r * vecs + v] = in[u];
-      }
+    p = x + r0 * a.x_stride + v0 * V + kept_vectors * hop;
+#pragma unroll 4
+    for (int k = kept_vectors; k < vectors; ++k, p += hop) sums = add_values(load_const<T, V>(p), sums);
+  } else {
+    for (int k = 0, r = r0, v = v0; k < vectors; ++k) {
+      const P in = load_const<T, V>(x + r * a.x_stride + v * V);
+      sums = add_values(in, sums);
+      if (k < kept_vectors) kept[threadIdx.x + k * step] = in;
       r += dr, v += dv;
       if (v >= vecs) ++r, v -= vecs;
     }
   }
-  // The thread's own mean, and its squares about it.
-  const float own = count > 0.f ? sum / count : 0.f;
-  float square = 0.f;
-  for (int r = r0, v = v0; walks && r < rows;) {
-    const P in = r < a.keep_rows ? kept[r * vecs + v] : load_const<T, V>(x + r * a.x_stride + v * V);
-    square = squares_about(in, own, square);
-    r += dr, v += dv;
-    if (v >= vecs) ++r, v -= vecs;
-  }
-  s_sum[threadIdx.x] = sum;
-  s_square[threadIdx.x] = square;
-  __syncthreads();
-  // A warp joins a group's threads: the sum gives the mean, then the squares
-  // move from the threads' means to it.
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int used = vecs <= kNormThreads ? step / vecs : 1, across = vecs <= kNormThreads ? group_vecs : kNormThreads;
-  for (int g = warp; g < groups; g += kNormThreads / 32) {
-    float total = 0.f;
-    for (int i = lane; i < used * across; i += 32) {
-      const int k = i / across, t = k * (vecs <= kNormThreads ? vecs : 0) + g * group_vecs + (i - k * across);
-      total += s_sum[t];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const float all = (float)rows * (float)a.width, mean = rows > 0 ? total / all : 0.f;
-    float squares = 0.f;
-    for (int i = lane; i < used * across; i += 32) {
-      const int k = i / across, t = k * (vecs <= kNormThreads ? vecs : 0) + g * group_vecs + (i - k * across);
-      // Vectors that thread t walked: every step-th of rows * vecs from t on.
-      const long long left = (long long)rows * vecs - t;
-      const float n = left > 0 ? (float)((left + step - 1) / step * V) : 0.f;
-      if (n > 0.f) {
-        const float d = s_sum[t] / n - mean;
-        squares += fmaf(n * d, d, s_square[t]);
+  // Squares of this thread's values about `mean`.
+  const auto squares_about = [&](float mean) {
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < kept_vectors; ++k) s = add_squares(kept[threadIdx.x + k * step], mean, s);
+    if (kept_vectors < vectors) {
+      int r = r0, v = v0;
+      for (int k = 0; k < vectors; ++k) {
+        if (k >= kept_vectors) s = add_squares(load_const<T, V>(x + r * a.x_stride + v * V), mean, s);
+        r += dr, v += dv;
+        if (v >= vecs) ++r, v -= vecs;
       }
     }
+    return s.x + s.y;
+  };
+  const float sum = sums.x + sums.y, all = (float)rows * (float)a.width;
+  if (groups == 1) {
+    const float mean = rows ? block_sum<NT>(sum, s_sum) / all : 0.f;
+    const float squares = block_sum<NT>(squares_about(mean), s_square);
+    if (threadIdx.x == 0) s_stats[0] = {all, mean, squares};
+  } else {
+    // A thread's squares are about its own mean. A warp joins a group's threads:
+    // the sum gives the mean, then the squares move to it.
+    const float n = (float)(vectors * V);
+    s_sum[threadIdx.x] = sum;
+    s_square[threadIdx.x] = vectors ? squares_about(sum / n) : 0.f;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int g = warp; g < groups; g += NT / 32) {
+      float total = 0.f, squares = 0.f;
+      for (int i = lane; i < dr * group_vecs; i += 32) {
+        const int k = i / group_vecs;
+        total += s_sum[k * vecs + g * group_vecs + i - k * group_vecs];
+      }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-    if (lane == 0) s_stats[g] = {all, mean, squares};
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const float mean = rows ? total / all : 0.f;
+      for (int i = lane; i < dr * group_vecs; i += 32) {
+        const int k = i / group_vecs, t = k * vecs + g * group_vecs + i - k * group_vecs;
+        // Vectors that thread t walked: rows k, k + dr, ...
+        const int walked = rows > k ? (rows - k - 1) / dr + 1 : 0;
+        if (walked) {
+          const float nt = (float)(walked * V), d = s_sum[t] / nt - mean;
+          squares += fmaf(nt * d, d, s_square[t]);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+      if (lane == 0) s_stats[g] = {all, mean, squares};
+    }
   }
   if (ctas > 1)
     cluster.sync();
@@ -311,86 +396,126 @@ __global__ void __launch_bounds__(kNormThreads) norm_kernel(const __grid_constan
   // Every CTA joins all of the cluster's, in order, into its own table.
   float* s_mean = s_sum;
   float* s_rstd = s_square;
-  if (threadIdx.x < groups) {  // at most kNormThreads
+  if (threadIdx.x < groups) {  // at most one a thread
     const int g = threadIdx.x;
-    Stats all = ctas > 1 ? cluster.map_shared_rank(s_stats, 0)[g] : s_stats[g];
-    for (int i = 1; i < ctas; ++i) all = join(all, cluster.map_shared_rank(s_stats, i)[g]);
+    Stats part[kMaxCtas];
+#pragma unroll
+    for (int i = 0; i < kMaxCtas; ++i)
+      if (i < ctas) part[i] = cluster.map_shared_rank(s_stats, i)[g];
+    Stats all = part[0];
+#pragma unroll
+    for (int i = 1; i < kMaxCtas; ++i)
+      if (i < ctas) all = join(all, part[i]);
     s_mean[g] = all.mean;
     s_rstd[g] = all.count > 0.f ? rsqrtf(all.squares / all.count + a.eps) : 0.f;
   }
+  if (ctas > 1) cluster_arrive();  // done with the others' statistics
   __syncthreads();
-  if (walks) {
-    if (dv == 0) {
-      // One vector of channels for good: its coefficients stay in registers.
-      const int g = v0 / group_vecs;
-      const float mean = s_mean[g], rstd = s_rstd[g];
+  if (dv == 0) {
+    // One vector of channels for good: its coefficients stay in registers.
+    const int g = min(v0 / group_vecs, groups - 1);
+    const float mean = s_mean[g];
+    NormChannels<V> ch;
+    if (vectors) ch.load(a, c0 + v0 * V);
+    ch.scale(s_rstd[g]);
+    T* p = y + r0 * a.y_stride + v0 * V;
+    const long long hop = dr * a.y_stride;
+#pragma unroll 2
+    for (int k = 0; k < kept_vectors; ++k, p += hop)
+      store_pack<T, V>(p, ch.apply(a.activation, kept[threadIdx.x + k * step], mean));
+    const T* from = x + (r0 + (long long)kept_vectors * dr) * a.x_stride + v0 * V;
+    for (int k = kept_vectors; k < vectors; ++k, p += hop, from += dr * a.x_stride)
+      store_pack<T, V>(p, ch.apply(a.activation, load_const<T, V>(from), mean));
+  } else {
+    for (int k = 0, r = r0, v = v0; k < vectors; ++k) {
+      const P in = k < kept_vectors ? kept[threadIdx.x + k * step] : load_const<T, V>(x + r * a.x_stride + v * V);
       NormChannels<V> ch;
-      if (r0 < rows) ch.load(a, c0 + v0 * V);
-#pragma unroll 4
-      for (int r = r0; r < rows; r += dr) {
-        const P in = r < a.keep_rows ? kept[r * vecs + v0] : load_const<T, V>(x + r * a.x_stride + v0 * V);
-        store_pack<T, V>(y + r * a.y_stride + v0 * V, ch.apply(a, in, mean, rstd));
-      }
-    } else {
-      for (int r = r0, v = v0; r < rows;) {
-        const P in = r < a.keep_rows ? kept[r * vecs + v] : load_const<T, V>(x + r * a.x_stride + v * V);
-        NormChannels<V> ch;
-        ch.load(a, c0 + v * V);
-        store_pack<T, V>(y + r * a.y_stride + v * V, ch.apply(a, in, s_mean[v / group_vecs], s_rstd[v / group_vecs]));
-        r += dr, v += dv;
-        if (v >= vecs) ++r, v -= vecs;
-      }
+      ch.load(a, c0 + v * V);
+      ch.scale(s_rstd[0]);
+      store_pack<T, V>(y + r * a.y_stride + v * V, ch.apply(a.activation, in, s_mean[0]));
+      r += dr, v += dv;
+      if (v >= vecs) ++r, v -= vecs;
     }
   }
-  if (ctas > 1) cluster.sync();  // no CTA leaves while another reads its statistics
+  if (ctas > 1) cluster_wait();  // no CTA leaves while another reads its statistics
 }
 
 constexpr int kMaxNormSmem = 200 * 1024;
+
+// Whether the device can place clusters of this size (more than 8 CTAs is not
+// guaranteed).
+bool clusters_fit(void (*kernel)(NormArgs), int ctas, int threads, size_t smem) {
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxNormSmem);
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) cudaGetLastError();
+  return clusters > 0;
+}
 
 template <typename T, int V>
 cudaError_t launch_rows(NormArgs a, cudaStream_t stream) {
   const int vecs = a.width / V;
   a.group_threads = 1;
-  while (a.group_threads < kNormThreads && a.group_threads < vecs) a.group_threads *= 2;
-  const long long per_block = kNormThreads / a.group_threads;
+  while (a.group_threads < kRowThreads && a.group_threads < vecs) a.group_threads *= 2;
+  const long long per_block = kRowThreads / a.group_threads;
   const long long blocks = ((long long)a.seq.rows * a.groups + per_block - 1) / per_block;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (vecs <= a.group_threads) return launch_op(norm_rows_kernel<T, V, 1>, (unsigned)blocks, kNormThreads, 0, stream, a);
+  if (vecs <= a.group_threads) return launch_op(norm_rows_kernel<T, V, 1>, (unsigned)blocks, kRowThreads, 0, stream, a);
   if (vecs <= 4 * a.group_threads)
-    return launch_op(norm_rows_kernel<T, V, 4>, (unsigned)blocks, kNormThreads, 0, stream, a);
-  return launch_op(norm_rows_kernel<T, V, 0>, (unsigned)blocks, kNormThreads, 0, stream, a);
+    return launch_op(norm_rows_kernel<T, V, 4>, (unsigned)blocks, kRowThreads, 0, stream, a);
+  return launch_op(norm_rows_kernel<T, V, 0>, (unsigned)blocks, kRowThreads, 0, stream, a);
+}
+
+template <typename T, int V, int NT>
+cudaError_t launch_cluster(const NormArgs& a, int ctas, size_t smem, cudaStream_t stream) {
+  const long long blocks = (long long)a.seq.n * a.blocks * ctas;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const auto kernel = norm_kernel<T, V, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxNormSmem);
+  if (e != cudaSuccess) return e;
+  if (ctas > 8 && (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
+    return e;
+  return launch_op(kernel, (unsigned)blocks, NT, smem, stream, a, (unsigned)ctas);
 }
 
 template <typename T, int V>
 cudaError_t launch_sequences(NormArgs a, cudaStream_t stream) {
   const int vecs = a.width / V;
-  // Whole groups, about 256 bytes of a row, one at least; several only while a
-  // thread can keep to one vector.
-  a.block_groups = 256 / (int)(a.width * sizeof(T));
-  if (a.block_groups < 1) a.block_groups = 1;
-  if (a.block_groups > a.groups) a.block_groups = a.groups;
-  while (a.block_groups > 1 && a.block_groups * vecs > kNormThreads) --a.block_groups;
+  // Whole groups, 64 bytes of a row where they are narrower: short rows leave
+  // a CTA's share small enough for several an SM without a larger cluster.
+  a.block_groups = std::max(1, std::min(a.groups, 64 / (int)(a.width * sizeof(T))));
+  while (a.block_groups > 1 && a.block_groups * vecs > kThreads) --a.block_groups;
   a.blocks = (a.groups + a.block_groups - 1) / a.block_groups;
-  const size_t row = (size_t)a.block_groups * a.width * sizeof(T);
+  const size_t row = (size_t)a.block_groups * a.width * sizeof(T), stats = a.block_groups * sizeof(Stats) + 16;
   // Shared memory for sequences of up to twice the mean length.
   const long long rows = a.seq.offsets ? std::min<long long>(a.seq.rows, 2LL * a.seq.rows / a.seq.n + 1) : a.seq.length;
-  // CTAs share a sequence while the GPU has room for more of them, and while a
-  // share is larger than a quarter of an SM's shared memory.
+  // CTAs share a sequence while there are fewer than two an SM, or while a share
+  // exceeds half an SM's shared memory.
   int ctas = 1;
-  while (ctas < 8 && rows >= 32 * ctas &&
-         ((long long)a.seq.n * a.blocks * ctas < 148 * 4 || (rows + ctas - 1) / ctas * row > kMaxNormSmem / 4))
+  while (ctas < kMaxCtas && rows >= 32 * ctas &&
+         ((long long)a.seq.n * a.blocks * ctas < 148 * 2 || (rows + ctas - 1) / ctas * row > kMaxNormSmem / 2))
     ctas *= 2;
-  const size_t stats = a.block_groups * sizeof(Stats) + 16;
-  const long long share = (rows + ctas - 1) / ctas;
-  a.keep_rows = (int)std::min<long long>(share, (kMaxNormSmem - stats) / row);
-  a.stats_at = (int)((a.keep_rows * row + 15) / 16 * 16);
-  const size_t smem = a.stats_at + stats;
-  const long long blocks = (long long)a.seq.n * a.blocks * ctas;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const cudaError_t e =
-      cudaFuncSetAttribute(norm_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxNormSmem);
-  if (e != cudaSuccess) return e;
-  return launch_op(norm_kernel<T, V>, (unsigned)blocks, kNormThreads, smem, stream, a, (unsigned)ctas);
+  const auto fit = [&] {
+    const long long share = (rows + ctas - 1) / ctas;
+    a.keep_rows = (int)std::min<long long>(share, (kMaxNormSmem - stats) / row);
+    a.stats_at = (int)((a.keep_rows * row + 15) / 16 * 16);
+    return a.stats_at + stats;
+  };
+  size_t smem = fit();
+  if (ctas > 8 && !clusters_fit(norm_kernel<T, V, kWideThreads>, ctas, kWideThreads, smem)) ctas = 8, smem = fit();
+  // Large shares, one CTA an SM, need its threads; small ones more CTAs.
+  if (smem > 64 * 1024 || ctas > 8) return launch_cluster<T, V, kWideThreads>(a, ctas, smem, stream);
+  return launch_cluster<T, V, kThreads>(a, ctas, smem, stream);
 }
 
 template <typename T, int V>

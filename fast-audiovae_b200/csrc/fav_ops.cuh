@@ -62,6 +62,24 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
   *reinterpret_cast<Pack<T, V>*>(p) = v;
 }
 
+// A pack from global into shared memory, asynchronously; without an
+// asynchronous copy of that size (2 bytes) at once.
+template <typename T, int V>
+__device__ __forceinline__ void copy_pack(Pack<T, V>* to, const T* from) {
+  if constexpr (sizeof(T) * V == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else if constexpr (sizeof(T) * V >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(sizeof(T) * V)
+                 : "memory");
+  else
+    *to = load_const<T, V>(from);
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Elements 2 i and 2 i + 1 of a pack in fp32, and back. V = 1: element 0 twice.
 template <typename T, int V>
 __device__ __forceinline__ float2 pair_of(const Pack<T, V>& p, int i) {
