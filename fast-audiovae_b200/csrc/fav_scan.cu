@@ -11,6 +11,18 @@
 // and one ex2 a state.
 #include "fav_ops.cuh"
 
+#ifndef MINB
+#define MINB 6
+#endif
+#ifndef QROWS
+#define QROWS 8
+#endif
+#ifndef SPLIT_BELOW
+#define SPLIT_BELOW 6
+#endif
+#ifndef SPLIT_WARPS
+#define SPLIT_WARPS 12
+#endif
 namespace fav {
 namespace {
 
@@ -22,15 +34,27 @@ struct ScanArgs {
   float* pool;
   Sequences seq;
   int channels, states, groups, softplus;
-  // Prompts: rows of a piece, pieces, 64-channel blocks of a group, and the
+  // Prompts: rows of a piece, pieces, blocks of channels of a group, and the
   // pieces' own results when sequences are split ([pieces][N][C], [pieces][C]).
-  int piece_rows, pieces, group_blocks;
+  int piece_rows, pieces, group_blocks, by_length;
   float* piece_state;
   float* piece_delta;
 };
 
-// log(1 + e^v), exact to a few fp32 roundings on both sides of zero.
-__device__ __forceinline__ float softplus_f32(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v| in (0, 1]; the logarithm is
+// 2 atanh(s), s = e / (2 + e) <= 1/3, whose series to s^13 is within 2e-8. No
+// digits are lost where e is small, as they would be in the logarithm of 1 + e.
+__device__ __forceinline__ float softplus_f32(float v) {
+  const float e = ex2_approx(-kLog2e * fabsf(v));
+  const float s = e * rcp_approx(2.f + e), q = s * s;
+  float p = fmaf(q, 0.153846154f, 0.181818182f);  // 2/13, 2/11, ...
+  p = fmaf(p, q, 0.222222222f);
+  p = fmaf(p, q, 0.285714286f);
+  p = fmaf(p, q, 0.4f);
+  p = fmaf(p, q, 0.666666667f);
+  p = fmaf(p, q, 2.f);
+  return fmaf(p, s, max_nan(v, 0.f));
+}
 
 __device__ __forceinline__ float delta_of(const ScanArgs& a, float dt, int c) {
   const float v = a.dt_bias ? dt + __ldg(a.dt_bias + c) : dt;
@@ -75,17 +99,27 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
     y[i] = 0.f;
   }
   const bool held = st.slot >= 0 && st.read >= 0, keep = live && st.slot >= 0;
-#pragma unroll 4
-  for (int n = l; n < a.states; n += L) {
-    const Pack<float, V> av = load_pack<float, V>(a.a + (size_t)n * a.channels + c);
-    Pack<float, V> h = held ? load_pack<float, V>(from + (size_t)n * a.channels) : Pack<float, V>{};
-    const float bn = to_f32(bp[n]), cn = to_f32(cp[n]);
+  constexpr int B = 8;  // states of a lane on their way at once
+  for (int n0 = l; n0 < a.states; n0 += B * L) {
+    Pack<float, V> h[B];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      h.v[i] = fmaf(ex2_approx(scale[i] * av.v[i]), h.v[i], dx[i] * bn);
-      y[i] = fmaf(h.v[i], cn, y[i]);
+    for (int k = 0; k < B; ++k) {
+      const int n = n0 + k * L;
+      h[k] = held && n < a.states ? load_pack<float, V>(from + (size_t)n * a.channels) : Pack<float, V>{};
     }
-    if (keep) store_pack<float, V>(to + (size_t)n * a.channels, h);
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int n = n0 + k * L;
+      if (n >= a.states) break;
+      const Pack<float, V> av = load_const<float, V>(a.a + (size_t)n * a.channels + c);
+      const float bn = to_f32(bp[n]), cn = to_f32(cp[n]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        h[k].v[i] = fmaf(ex2_approx(scale[i] * av.v[i]), h[k].v[i], dx[i] * bn);
+        y[i] = fmaf(h[k].v[i], cn, y[i]);
+      }
+      if (keep) store_pack<float, V>(to + (size_t)n * a.channels, h[k]);
+    }
   }
 #pragma unroll
   for (int o = W; o < 32; o *= 2)
@@ -105,15 +139,16 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
 
 // ----------------------------------------------------------------- prompts
 // A block owns CH neighbouring channels of one group over one piece (a whole
-// sequence, or a run of its rows). L lanes share a channel, eight states each
-// in registers. Per tile of 32 rows all threads first form delta and delta * x
-// (the softplus once per value, not once per state) and widen b and c in shared
-// memory; then each thread steps through the rows, and y replaces delta in
-// place; then all threads add d * x, gate and store.
+// sequence, or a run of its rows). L lanes share a channel, S states each in
+// registers as pairs; every lane forms the channel's delta, so that nothing but
+// b and c passes through shared memory in fp32. Tiles of 16 rows of x, dt and z
+// are copied ahead of their use (cp.async) into two buffers, and y takes x's
+// place in them until the tile is stored.
 //
-// Bound by ex2: T * C * N of them at 16 a clock and SM.
-constexpr int kTileRows = 32;
-constexpr int kLaneStates = 8;
+// Bound by ex2: T * C * N of them at 16 a clock and SM, and four more a value
+// for softplus and gate.
+constexpr int kTileRows = 16;
+constexpr int kBlockChannels = 64;
 
 // A piece: rows [begin, end) of sequence ``seq``; pieces ``first``.. of the
 // same sequence precede it.
@@ -163,20 +198,51 @@ __device__ __forceinline__ Piece piece_at(const ScanArgs& a, int p) {
   return r;
 }
 
+// The sequence that is number `rank` by length, longest first (n <= NT). In that
+// order every SM gets long and short ones alike: 33 prompts of up to 750 rows,
+// all resident at once, took as long as the SM with the most rows.
+template <int NT>
+__device__ __forceinline__ int sequence_by_length(const Sequences& q, int rank) {
+  __shared__ int s_length[NT], s_pick;
+  const int t = threadIdx.x;
+  int length = -1;
+  if (t < q.n) {
+    const Span sp = span_of(q, t);
+    length = max(sp.end - sp.begin, -1);
+  }
+  s_length[t] = length;
+  __syncthreads();
+  if (t < q.n) {
+    int before = 0;
+    for (int j = 0; j < q.n; ++j) before += s_length[j] > length || (s_length[j] == length && j < t);
+    if (before == rank) s_pick = t;
+  }
+  __syncthreads();
+  return s_pick;
+}
+
 // PARTIAL: the state a piece reaches by itself and its sum of delta, for the
 // pieces behind it; no y.
-template <typename T, int V, int L, int CH, bool PARTIAL>
-__global__ void __launch_bounds__(CH* L) scan_kernel(const __grid_constant__ ScanArgs a) {
-  constexpr int NT = CH * L, S = kLaneStates, NP = S * L, R = kTileRows;
-  constexpr int VPT = (R * CH / V + NT - 1) / NT;  // vectors of a tile per thread
-  __shared__ __align__(16) float s_delta[R][CH];
-  __shared__ __align__(16) float s_dx[R][CH];
-  __shared__ __align__(16) float s_b[R][NP];
-  __shared__ __align__(16) float s_c[PARTIAL ? 1 : R][NP];
+template <typename T, bool WIDE, int S, int L, bool PARTIAL>
+__global__ void __launch_bounds__(kBlockChannels* L, MINB / L > 0 ? MINB / L : 1) scan_kernel(const __grid_constant__ ScanArgs a) {
+  constexpr int CH = kBlockChannels, R = kTileRows, Q = QROWS, NT = CH * L, NP = S * L, H = S / 2;
+  constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
+  constexpr int kMaps = R * NP / NT;  // values of b (and of c) of a tile per thread
+  static_assert(kMaps * NT == R * NP, "tile split");
+  struct Tile {
+    T x[R][CH], dt[R][CH], z[PARTIAL ? 1 : R][CH];
+  };
+  struct Maps {
+    float b[R][NP], c[PARTIAL ? 1 : R][NP];
+  };
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  Tile* s_tile = reinterpret_cast<Tile*>(s_raw);                    // two
+  Maps* s_maps = reinterpret_cast<Maps*>(s_raw + 2 * sizeof(Tile));  // two
   grid_dependency_sync();
   const Sequences& q = a.seq;
   const int blocks = a.group_blocks * a.groups;
-  const int p = blockIdx.x / blocks, cb = blockIdx.x - p * blocks;
+  const int turn = blockIdx.x / blocks, cb = blockIdx.x - turn * blocks;
+  const int p = a.by_length && !PARTIAL ? sequence_by_length<NT>(q, turn) : turn;
   const int g = cb / a.group_blocks, width = a.channels / a.groups;
   const int c_in = (cb - g * a.group_blocks) * CH;  // first channel inside the group
   const int c0 = g * width + c_in, count = min(CH, width - c_in);
@@ -188,136 +254,190 @@ __global__ void __launch_bounds__(CH* L) scan_kernel(const __grid_constant__ Sca
   if (!pc.ok || (PARTIAL && pc.last)) return;
   const SlotRef st = slot_of(q, pc.seq);
   if (st.bad) return;
+
+  const T* xb = static_cast<const T*>(a.x) + c0;
+  const T* db = static_cast<const T*>(a.dt) + c0;
+  const T* zb = static_cast<const T*>(a.z) + c0;
+  const T* bb = static_cast<const T*>(a.b) + g * a.b_group;
+  const T* cc = static_cast<const T*>(a.c) + g * a.c_group;
+  const bool gate = !PARTIAL && a.z != nullptr;
+  T maps_b[kMaps], maps_c[kMaps];
+  // Where this thread's vectors of a tile lie, kVecs of them kHop rows apart, and
+  // its values of b and c, kMaps of them kMapHop rows apart.
+  constexpr int kAcross = CH / V, kVecs = (R * kAcross + NT - 1) / NT, kHop = NT / kAcross, kMapHop = NT / NP;
+  static_assert(NT % kAcross == 0 && NT % NP == 0, "a thread keeps to one column");
+  const int vr = threadIdx.x / kAcross, vi = threadIdx.x % kAcross * V;
+  const int mr = threadIdx.x / NP, mn = threadIdx.x % NP;
+  const bool v_in = vi < count, m_in = mn < a.states;
+  const T* px = xb + (pc.begin + vr) * a.x_stride + vi;
+  const T* pd = db + (pc.begin + vr) * a.dt_stride + vi;
+  const T* pz = gate ? zb + (pc.begin + vr) * a.z_stride + vi : nullptr;
+  const T* pb = bb + (pc.begin + mr) * a.b_stride + mn;
+  const T* pq = cc + (pc.begin + mr) * a.c_stride + mn;
+  // Starts the copies of the next tile, of `rows` rows, into buffer `to`, and its
+  // b and c into registers.
+  const auto fetch = [&](int rows, int to) {
+    Tile& tile = s_tile[to];
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int r = vr + k * kHop;
+      if (v_in && r < rows) {
+        copy_pack<T, V>(reinterpret_cast<Pack<T, V>*>(&tile.x[r][vi]), px + k * kHop * a.x_stride);
+        copy_pack<T, V>(reinterpret_cast<Pack<T, V>*>(&tile.dt[r][vi]), pd + k * kHop * a.dt_stride);
+        if constexpr (!PARTIAL)
+          if (gate) copy_pack<T, V>(reinterpret_cast<Pack<T, V>*>(&tile.z[r][vi]), pz + k * kHop * a.z_stride);
+      }
+    }
+    copy_commit();
+#pragma unroll
+    for (int k = 0; k < kMaps; ++k) {
+      const bool in = m_in && mr + k * kMapHop < rows;
+      maps_b[k] = in ? pb[k * kMapHop * a.b_stride] : from_f32<T>(0.f);
+      if constexpr (!PARTIAL) maps_c[k] = in ? pq[k * kMapHop * a.c_stride] : from_f32<T>(0.f);
+    }
+    px += R * a.x_stride, pd += R * a.dt_stride, pb += R * a.b_stride;
+    if constexpr (!PARTIAL) pz += gate ? R * a.z_stride : 0, pq += R * a.c_stride;
+  };
+  if (pc.begin < pc.end) fetch(min(R, pc.end - pc.begin), 0);
+
   const int ch = threadIdx.x / L, l = threadIdx.x % L;
   const bool mine = ch < count;
   const int c = c0 + (mine ? ch : 0);
   const size_t table = (size_t)a.states * a.channels;
+  // State j of this lane is number l * S + j.
+  const auto each = [&](auto&& f) {
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (l * S + j < a.states) f(j, (size_t)(l * S + j) * a.channels);
+  };
   float decay[S], h[S];
 #pragma unroll
-  for (int j = 0; j < S; ++j) {
-    const int n = l * S + j;
-    decay[j] = n < a.states ? __ldg(a.a + (size_t)n * a.channels + c) * kLog2e : 0.f;
-    h[j] = 0.f;
-  }
+  for (int j = 0; j < S; ++j) decay[j] = h[j] = 0.f;
+  // (finite, so that a row of delta = 0 keeps the state even where a is not)
+  each([&](int j, size_t at) { decay[j] = max_nan(__ldg(a.a + at + c) * kLog2e, -3e38f); });
   if (p == pc.first) {
     if (st.slot >= 0 && st.read >= 0) {
       const float* from = a.pool + (2 * (size_t)st.slot + st.read) * table + c;
-#pragma unroll
-      for (int j = 0; j < S; ++j)
-        if (l * S + j < a.states) h[j] = from[(size_t)(l * S + j) * a.channels];
+      each([&](int j, size_t at) { h[j] = from[at]; });
     }
   } else if (!PARTIAL) {
     // Join the pieces before this one, in order.
-    for (int k = pc.first; k < p; ++k) {
-      const float sum = a.piece_delta[(size_t)k * a.channels + c];
-      const float* from = a.piece_state + (size_t)k * table + c;
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        const float v = l * S + j < a.states ? from[(size_t)(l * S + j) * a.channels] : 0.f;
-        h[j] = k == pc.first ? v : fmaf(ex2_approx(sum * decay[j]), h[j], v);
-      }
+    const float* from = a.piece_state + (size_t)pc.first * table + c;
+    const float* sums = a.piece_delta + (size_t)pc.first * a.channels + c;
+    each([&](int j, size_t at) { h[j] = from[at]; });
+#pragma unroll 2
+    for (int k = pc.first + 1; k < p; ++k) {
+      from += table;
+      sums += a.channels;
+      const float sum = *sums;
+      each([&](int j, size_t at) { h[j] = fmaf(ex2_approx(sum * decay[j]), h[j], from[at]); });
     }
   }
+  const float bias = a.dt_bias ? __ldg(a.dt_bias + c) : 0.f, skip = !PARTIAL && a.d ? __ldg(a.d + c) : 0.f;
+  float2 decay2[H], h2[H];
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    decay2[j] = make_float2(decay[2 * j], decay[2 * j + 1]);
+    h2[j] = make_float2(h[2 * j], h[2 * j + 1]);
+  }
+  T* py = static_cast<T*>(a.y) + c0 + (pc.begin + vr) * a.y_stride + vi;
   float total = 0.f;  // PARTIAL: sum of delta
-  const T* xb = static_cast<const T*>(a.x) + c0;
-  const T* db = static_cast<const T*>(a.dt) + c0;
-  const T* zb = static_cast<const T*>(a.z) + c0;
-  T* yb = static_cast<T*>(a.y) + c0;
-  const T* bb = static_cast<const T*>(a.b) + g * a.b_group;
-  const T* cc = static_cast<const T*>(a.c) + g * a.c_group;
-  for (int t0 = pc.begin; t0 < pc.end; t0 += R) {
+  int buffer = 0;
+  for (int t0 = pc.begin; t0 < pc.end; t0 += R, buffer ^= 1) {
     const int rows = min(R, pc.end - t0);
-    Pack<T, V> xv[VPT];
+    Tile& tile = s_tile[buffer];
+    Maps& maps = s_maps[buffer];
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int e = (k * NT + threadIdx.x) * V, r = e / CH, i = e % CH;
-      if (R * CH / V % NT && r >= R) continue;
-      const bool in = r < rows && i < count;
-      Pack<T, V> dv{};
-      xv[k] = Pack<T, V>{};
-      if (in) {
-        xv[k] = load_pack<T, V>(xb + (t0 + r) * a.x_stride + i);
-        dv = load_pack<T, V>(db + (t0 + r) * a.dt_stride + i);
-      }
-      Pack<float, V> delta, dx;
-#pragma unroll
-      for (int u = 0; u < V; ++u) {
-        // A row behind the last: delta = 0 keeps every state as it is.
-        delta.v[u] = in ? delta_of(a, to_f32(dv.v[u]), c0 + i + u) : 0.f;
-        dx.v[u] = in ? delta.v[u] * to_f32(xv[k].v[u]) : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < V; ++u) {
-        s_delta[r][i + u] = delta.v[u];
-        s_dx[r][i + u] = dx.v[u];
-      }
+    for (int k = 0; k < kMaps; ++k) {
+      maps.b[mr + k * kMapHop][mn] = to_f32(maps_b[k]);
+      if constexpr (!PARTIAL) maps.c[mr + k * kMapHop][mn] = to_f32(maps_c[k]);
     }
-    for (int e = threadIdx.x; e < R * NP; e += NT) {
-      const int r = e / NP, n = e % NP;
-      const bool in = r < rows && n < a.states;
-      s_b[r][n] = in ? to_f32(bb[(t0 + r) * a.b_stride + n]) : 0.f;
-      if (!PARTIAL) s_c[r][n] = in ? to_f32(cc[(t0 + r) * a.c_stride + n]) : 0.f;
-    }
+    copy_wait<0>();
     __syncthreads();
-#pragma unroll 4
-    for (int r = 0; r < R; ++r) {
-      const float delta = s_delta[r][ch], dx = s_dx[r][ch];
-      float y = 0.f;
+    if (t0 + R < pc.end) fetch(min(R, pc.end - t0 - R), buffer ^ 1);
+    // Q rows at a time: their deltas together, then the states row by row, then
+    // their outputs together, so that only the states' own chain is serial. A row
+    // behind the last has delta = 0 and keeps every state as it is.
+    for (int r0 = 0; r0 < rows; r0 += Q) {
+      // Lane l forms delta of the rows u with u % L = l for the channel's others.
+      float own_delta[Q / L], own_dx[Q / L], y[Q];
 #pragma unroll
-      for (int j = 0; j < S; j += 4) {
-        const float4 bv = *reinterpret_cast<const float4*>(&s_b[r][l * S + j]);
-        h[j] = fmaf(ex2_approx(delta * decay[j]), h[j], dx * bv.x);
-        h[j + 1] = fmaf(ex2_approx(delta * decay[j + 1]), h[j + 1], dx * bv.y);
-        h[j + 2] = fmaf(ex2_approx(delta * decay[j + 2]), h[j + 2], dx * bv.z);
-        h[j + 3] = fmaf(ex2_approx(delta * decay[j + 3]), h[j + 3], dx * bv.w);
-        if constexpr (!PARTIAL) {
-          const float4 cv = *reinterpret_cast<const float4*>(&s_c[r][l * S + j]);
-          y = fmaf(h[j], cv.x, y);
-          y = fmaf(h[j + 1], cv.y, y);
-          y = fmaf(h[j + 2], cv.z, y);
-          y = fmaf(h[j + 3], cv.w, y);
+      for (int k = 0; k < Q / L; ++k) {
+        const int r = r0 + k * L + l;
+        const float v = to_f32(tile.dt[r][ch]) + bias;
+        own_delta[k] = r < rows ? (a.softplus ? softplus_f32(v) : v) : 0.f;
+        own_dx[k] = r < rows ? own_delta[k] * to_f32(tile.x[r][ch]) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < Q; ++u) {
+        float delta = own_delta[u / L], dx = own_dx[u / L];
+        if constexpr (L > 1) {
+          delta = __shfl_sync(0xffffffffu, delta, u % L, L);
+          dx = __shfl_sync(0xffffffffu, dx, u % L, L);
+        }
+        const float2 delta2 = make_float2(delta, delta), dx2 = make_float2(dx, dx);
+        float2 y2 = make_float2(0.f, 0.f), y3 = y2;
+#pragma unroll
+        for (int j = 0; j < H; j += 2) {
+          const float4 bv = *reinterpret_cast<const float4*>(&maps.b[r0 + u][l * S + 2 * j]);
+          const float2 p0 = f2mul(delta2, decay2[j]), p1 = f2mul(delta2, decay2[j + 1]);
+          h2[j] = f2fma(make_float2(ex2_approx(p0.x), ex2_approx(p0.y)), h2[j], f2mul(dx2, make_float2(bv.x, bv.y)));
+          h2[j + 1] =
+              f2fma(make_float2(ex2_approx(p1.x), ex2_approx(p1.y)), h2[j + 1], f2mul(dx2, make_float2(bv.z, bv.w)));
+          if constexpr (!PARTIAL) {
+            const float4 cv = *reinterpret_cast<const float4*>(&maps.c[r0 + u][l * S + 2 * j]);
+            y2 = f2fma(h2[j], make_float2(cv.x, cv.y), y2);
+            y3 = f2fma(h2[j + 1], make_float2(cv.z, cv.w), y3);
+          }
+        }
+        if constexpr (PARTIAL) {
+          total += delta;
+        } else {
+          y2 = f2add(y2, y3);
+          y[u] = y2.x + y2.y;
         }
       }
-      if constexpr (PARTIAL) {
-        total += delta;
-      } else {
+      if constexpr (!PARTIAL) {
+        // Sums over the lanes, row u's to lane u % L: each step halves the rows that
+        // a lane has left.
 #pragma unroll
-        for (int o = 1; o < L; o *= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-        if (l == 0) s_delta[r][ch] = y;  // the channel's lanes have all read delta: they are in one warp
+        for (int o = 1, left = Q; o < L; o *= 2, left /= 2)
+#pragma unroll
+          for (int k = 0; k < left / 2; ++k) {
+            const bool odd = l & o;
+            const float send = odd ? y[2 * k] : y[2 * k + 1];
+            y[k] = (odd ? y[2 * k + 1] : y[2 * k]) + __shfl_xor_sync(0xffffffffu, send, o);
+          }
+#pragma unroll
+        for (int k = 0; k < Q / L; ++k) {
+          const int r = r0 + k * L + l;
+          float v = fmaf(skip, to_f32(tile.x[r][ch]), y[k]);
+          if (gate) v *= silu(to_f32(tile.z[r][ch]));
+          tile.x[r][ch] = from_f32<T>(v);  // read by this lane alone
+        }
       }
     }
-    __syncthreads();
     if constexpr (!PARTIAL) {
-#pragma unroll
-      for (int k = 0; k < VPT; ++k) {
-        const int e = (k * NT + threadIdx.x) * V, r = e / CH, i = e % CH;
-        if (r >= rows || i >= count) continue;
-        Pack<T, V> out, zv{};
-        if (a.z) zv = load_pack<T, V>(zb + (t0 + r) * a.z_stride + i);
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-          const float y = s_delta[r][i + u];
-          float v = a.d ? fmaf(__ldg(a.d + c0 + i + u), to_f32(xv[k].v[u]), y) : y;
-          if (a.z) v *= silu(to_f32(zv.v[u]));
-          out.v[u] = from_f32<T>(v);
-        }
-        store_pack<T, V>(yb + (t0 + r) * a.y_stride + i, out);
-      }
       __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int r = vr + k * kHop;
+        if (v_in && r < rows)
+          store_pack<T, V>(py + k * kHop * a.y_stride, *reinterpret_cast<const Pack<T, V>*>(&tile.x[r][vi]));
+      }
+      py += R * a.y_stride;
     }
   }
   if (!mine) return;
+#pragma unroll
+  for (int j = 0; j < H; ++j) h[2 * j] = h2[j].x, h[2 * j + 1] = h2[j].y;
   if (PARTIAL) {
     float* to = a.piece_state + (size_t)p * table + c;
-#pragma unroll
-    for (int j = 0; j < S; ++j)
-      if (l * S + j < a.states) to[(size_t)(l * S + j) * a.channels] = h[j];
+    each([&](int j, size_t at) { to[at] = h[j]; });
     if (l == 0) a.piece_delta[(size_t)p * a.channels + c] = total;
   } else if (pc.last && st.slot >= 0) {
     float* to = a.pool + (2 * (size_t)st.slot + st.write) * table + c;
-#pragma unroll
-    for (int j = 0; j < S; ++j)
-      if (l * S + j < a.states) to[(size_t)(l * S + j) * a.channels] = h[j];
+    each([&](int j, size_t at) { to[at] = h[j]; });
   }
 }
 
@@ -335,39 +455,57 @@ cudaError_t launch_step(const ScanArgs& a, cudaStream_t stream) {
   return launch_op(scan_step_kernel<T, V, 1>, (unsigned)blocks, kStepThreads, 0, stream, a);
 }
 
-template <typename T, int V, int L, int CH>
+template <typename T, bool WIDE, int S, int L, bool PARTIAL>
+cudaError_t launch_scan(const ScanArgs& a, unsigned blocks, cudaStream_t stream) {
+  constexpr int R = kTileRows;
+  const size_t tile = (size_t)R * kBlockChannels * sizeof(T), maps = (size_t)R * S * L * sizeof(float);
+  const size_t smem = PARTIAL ? 2 * (2 * tile + kBlockChannels * sizeof(T) + maps + S * L * sizeof(float))
+                              : 2 * (3 * tile + 2 * maps);
+  const auto kernel = scan_kernel<T, WIDE, S, L, PARTIAL>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_op(kernel, blocks, kBlockChannels * L, smem, stream, a);
+}
+
+template <typename T, bool WIDE, int S, int L>
 cudaError_t launch_pieces(const ScanArgs& a, cudaStream_t stream) {
   const long long blocks = (long long)a.pieces * a.group_blocks * a.groups;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (a.piece_state) {
-    const cudaError_t e = launch_op(scan_kernel<T, V, L, CH, true>, (unsigned)blocks, CH * L, 0, stream, a);
+    const cudaError_t e = launch_scan<T, WIDE, S, L, true>(a, (unsigned)blocks, stream);
     if (e != cudaSuccess) return e;
   }
-  return launch_op(scan_kernel<T, V, L, CH, false>, (unsigned)blocks, CH * L, 0, stream, a);
+  return launch_scan<T, WIDE, S, L, false>(a, (unsigned)blocks, stream);
 }
 
+// Lanes of a channel: 8 states each, 16 above 64.
 int lanes_for(int states) {
   int lanes = 1;
-  while (lanes * kLaneStates < states) lanes *= 2;
+  while (lanes < 8 && lanes * 8 < states) lanes *= 2;
   return lanes;
 }
-int block_channels(int lanes) { return lanes <= 8 ? 64 : 32; }
 
-template <typename T, int V>
+template <typename T, bool WIDE>
 cudaError_t launch_lanes(const ScanArgs& a, cudaStream_t stream) {
   switch (lanes_for(a.states)) {
-    case 1: return launch_pieces<T, V, 1, 64>(a, stream);
-    case 2: return launch_pieces<T, V, 2, 64>(a, stream);
-    case 4: return launch_pieces<T, V, 4, 64>(a, stream);
-    case 8: return launch_pieces<T, V, 8, 64>(a, stream);
-    default: return launch_pieces<T, V, 16, 32>(a, stream);
+    case 1: return launch_pieces<T, WIDE, 8, 1>(a, stream);
+#ifdef L16
+    case 2: return launch_pieces<T, WIDE, 16, 1>(a, stream);
+#else
+    case 2: return launch_pieces<T, WIDE, 8, 2>(a, stream);
+#endif
+    case 4: return launch_pieces<T, WIDE, 8, 4>(a, stream);
+    default: break;
   }
+  return a.states <= 64 ? launch_pieces<T, WIDE, 8, 8>(a, stream) : launch_pieces<T, WIDE, 16, 8>(a, stream);
 }
 
 template <typename T>
 cudaError_t launch_type(const ScanArgs& a, bool step, bool wide, cudaStream_t stream) {
   if (step) return wide ? launch_step<T, 4>(a, stream) : launch_step<T, 1>(a, stream);
-  return wide ? launch_lanes<T, 4>(a, stream) : launch_lanes<T, 1>(a, stream);
+  return wide ? launch_lanes<T, true>(a, stream) : launch_lanes<T, false>(a, stream);
 }
 
 // How the rows are cut: piece_rows and pieces.
@@ -377,19 +515,18 @@ struct Split {
 };
 
 Split split_of(const fav_scan_args& c, const Sequences& q) {
-  const int lanes = lanes_for(c.states), ch = block_channels(lanes);
   const int width = c.channels / c.groups;
-  const long long blocks = (long long)c.groups * ((width + ch - 1) / ch);
-  const int warps = ch * lanes / 32;
+  const long long blocks = (long long)c.groups * ((width + kBlockChannels - 1) / kBlockChannels);
+  const int warps = kBlockChannels * lanes_for(c.states) / 32;
   // A split scan forms every decay twice. It pays where whole sequences would
   // leave most of the GPU idle.
   const long long have = blocks * q.n * warps;
   const long long longest = q.offsets ? q.rows : q.length;
-  if (have >= 148 * 8 || longest <= 2 * kTileRows) return {q.rows + 1, q.n, false};
-  long long want = (148 * 24 + blocks * warps - 1) / (blocks * warps);
+  if (have >= 148 * SPLIT_BELOW || longest <= 4 * kTileRows) return {q.rows + 1, q.n, false};
+  const long long want = (148 * SPLIT_WARPS + blocks * warps - 1) / (blocks * warps);
   long long rows = (q.rows + want - 1) / want;
   rows = (rows + kTileRows - 1) / kTileRows * kTileRows;
-  if (rows < kTileRows) rows = kTileRows;
+  if (rows < 2 * kTileRows) rows = 2 * kTileRows;
   if (q.offsets) return {(int)rows, (int)(q.rows / rows) + q.n, true};
   const long long per = (q.length - 1) / rows + 1;
   return {(int)rows, (int)(per * q.n), per > 1};
@@ -431,15 +568,17 @@ cudaError_t launch_selective_scan(const fav_scan_args& c, const Sequences& seq, 
   if (seq.n == 0) return cudaSuccess;
   const bool step = !seq.offsets && seq.length == 1;
   const int elem = elem_bytes(c.type), width = c.channels / c.groups;
-  const bool wide = width % 4 == 0 && aligned_for(c.x, c.x_stride, elem, 4) && aligned_for(c.dt, c.dt_stride, elem, 4) &&
-                    aligned_for(c.z, c.z_stride, elem, 4) && aligned_for(c.y, c.y_stride, elem, 4) &&
-                    aligned_for(c.a, 0, 4, 4) && aligned_for(c.state_pool, 0, 4, 4);
+  // Steps move four channels at a time, prompts 16 bytes.
+  const int v = step ? 4 : 16 / elem;
+  const bool wide = width % v == 0 && aligned_for(c.x, c.x_stride, elem, v) && aligned_for(c.dt, c.dt_stride, elem, v) &&
+                    aligned_for(c.z, c.z_stride, elem, v) && aligned_for(c.y, c.y_stride, elem, v) &&
+                    (!step || (aligned_for(c.a, 0, 4, 4) && aligned_for(c.state_pool, 0, 4, 4)));
   if (!step) {
     const Split s = split_of(c, seq);
     a.piece_rows = s.piece_rows;
     a.pieces = s.pieces;
-    const int ch = block_channels(lanes_for(c.states));
-    a.group_blocks = (width + ch - 1) / ch;
+    a.by_length = seq.offsets && !s.split && seq.n <= kBlockChannels;
+    a.group_blocks = (width + kBlockChannels - 1) / kBlockChannels;
     if (s.split) {
       a.piece_state = static_cast<float*>(c.workspace);
       a.piece_delta = a.piece_state + (size_t)s.pieces * c.channels * c.states;
