@@ -9,20 +9,10 @@
 // or from zero and goes to the slot's other table. All of it runs in fp32 and
 // y rounds once to its type. The decay is 2^(delta * a * log2 e): one multiply
 // and one ex2 a state.
+#include <algorithm>
+
 #include "fav_ops.cuh"
 
-#ifndef MINB
-#define MINB 6
-#endif
-#ifndef QROWS
-#define QROWS 8
-#endif
-#ifndef SPLIT_BELOW
-#define SPLIT_BELOW 6
-#endif
-#ifndef SPLIT_WARPS
-#define SPLIT_WARPS 12
-#endif
 namespace fav {
 namespace {
 
@@ -65,7 +55,9 @@ __device__ __forceinline__ float delta_of(const ScanArgs& a, float dt, int c) {
 // One row per stream. Reading and writing the states is the whole cost (8 * N
 // bytes a channel), so a thread moves V = 4 neighbouring channels of a state
 // with 16-byte accesses; L lanes of a warp share a channel's states where
-// there are too few channels and streams to fill the GPU.
+// there are too few channels and streams to fill the GPU. 512 streams of 2048 x 16
+// take 34 us, 60 % of the copy rate. (Holding `a` in registers over several
+// streams took 51 us: the registers cost more warps than the reads of `a` time.)
 constexpr int kStepThreads = 128;
 
 template <typename T, int V, int L>
@@ -99,7 +91,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
     y[i] = 0.f;
   }
   const bool held = st.slot >= 0 && st.read >= 0, keep = live && st.slot >= 0;
-  constexpr int B = 8;  // states of a lane on their way at once
+  constexpr int B = 4;  // states of a lane on their way at once (eight: fewer warps, 36 us)
   for (int n0 = l; n0 < a.states; n0 += B * L) {
     Pack<float, V> h[B];
 #pragma unroll
@@ -224,8 +216,8 @@ __device__ __forceinline__ int sequence_by_length(const Sequences& q, int rank) 
 // PARTIAL: the state a piece reaches by itself and its sum of delta, for the
 // pieces behind it; no y.
 template <typename T, bool WIDE, int S, int L, bool PARTIAL>
-__global__ void __launch_bounds__(kBlockChannels* L, MINB / L > 0 ? MINB / L : 1) scan_kernel(const __grid_constant__ ScanArgs a) {
-  constexpr int CH = kBlockChannels, R = kTileRows, Q = QROWS, NT = CH * L, NP = S * L, H = S / 2;
+__global__ void __launch_bounds__(kBlockChannels* L, L == 2 ? 3 : 1) scan_kernel(const __grid_constant__ ScanArgs a) {
+  constexpr int CH = kBlockChannels, R = kTileRows, Q = 8, NT = CH * L, NP = S * L, H = S / 2;
   constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
   constexpr int kMaps = R * NP / NT;  // values of b (and of c) of a tile per thread
   static_assert(kMaps * NT == R * NP, "tile split");
@@ -325,7 +317,7 @@ __global__ void __launch_bounds__(kBlockChannels* L, MINB / L > 0 ? MINB / L : 1
     const float* from = a.piece_state + (size_t)pc.first * table + c;
     const float* sums = a.piece_delta + (size_t)pc.first * a.channels + c;
     each([&](int j, size_t at) { h[j] = from[at]; });
-#pragma unroll 2
+#pragma unroll 4
     for (int k = pc.first + 1; k < p; ++k) {
       from += table;
       sums += a.channels;
@@ -444,13 +436,10 @@ __global__ void __launch_bounds__(kBlockChannels* L, MINB / L > 0 ? MINB / L : 1
 template <typename T, int V>
 cudaError_t launch_step(const ScanArgs& a, cudaStream_t stream) {
   const long long items = (long long)a.seq.n * (a.channels / V);
-  // Lanes per channel vector: more while the call has under 1024 threads an SM
-  // and every lane still has states.
-  int lanes = 1;
-  while (lanes < 16 && items * lanes < 148 * 1024 && lanes * 4 <= a.states) lanes *= 4;
+  // Four lanes per channel vector while one would leave an SM under 1024 threads.
+  const int lanes = items < 148 * 1024 ? 4 : 1;
   const long long blocks = (items * lanes + kStepThreads - 1) / kStepThreads;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (lanes == 16) return launch_op(scan_step_kernel<T, V, 16>, (unsigned)blocks, kStepThreads, 0, stream, a);
   if (lanes == 4) return launch_op(scan_step_kernel<T, V, 4>, (unsigned)blocks, kStepThreads, 0, stream, a);
   return launch_op(scan_step_kernel<T, V, 1>, (unsigned)blocks, kStepThreads, 0, stream, a);
 }
@@ -480,22 +469,20 @@ cudaError_t launch_pieces(const ScanArgs& a, cudaStream_t stream) {
   return launch_scan<T, WIDE, S, L, false>(a, (unsigned)blocks, stream);
 }
 
-// Lanes of a channel: 8 states each, 16 above 64.
+// Lanes of a channel: 4 states each up to 8, 8 up to 64, 16 above. (16 states in
+// one lane take a seventh fewer instructions, but leave too few warps: ragged
+// prompts of 16 states 238 us, against 170 us with two lanes.)
 int lanes_for(int states) {
-  int lanes = 1;
+  int lanes = 2;
   while (lanes < 8 && lanes * 8 < states) lanes *= 2;
   return lanes;
 }
 
 template <typename T, bool WIDE>
 cudaError_t launch_lanes(const ScanArgs& a, cudaStream_t stream) {
+  if (a.states <= 8) return launch_pieces<T, WIDE, 4, 2>(a, stream);
   switch (lanes_for(a.states)) {
-    case 1: return launch_pieces<T, WIDE, 8, 1>(a, stream);
-#ifdef L16
-    case 2: return launch_pieces<T, WIDE, 16, 1>(a, stream);
-#else
     case 2: return launch_pieces<T, WIDE, 8, 2>(a, stream);
-#endif
     case 4: return launch_pieces<T, WIDE, 8, 4>(a, stream);
     default: break;
   }
@@ -518,12 +505,13 @@ Split split_of(const fav_scan_args& c, const Sequences& q) {
   const int width = c.channels / c.groups;
   const long long blocks = (long long)c.groups * ((width + kBlockChannels - 1) / kBlockChannels);
   const int warps = kBlockChannels * lanes_for(c.states) / 32;
-  // A split scan forms every decay twice. It pays where whole sequences would
-  // leave most of the GPU idle.
+  // A split scan forms every decay twice: it pays where whole sequences leave an
+  // SM fewer than six warps. Twelve an SM then: fewer leave it idle (one prompt of
+  // 6000 x 1024: 88 us, with eight 130), more pieces take longer to join.
   const long long have = blocks * q.n * warps;
   const long long longest = q.offsets ? q.rows : q.length;
-  if (have >= 148 * SPLIT_BELOW || longest <= 4 * kTileRows) return {q.rows + 1, q.n, false};
-  const long long want = (148 * SPLIT_WARPS + blocks * warps - 1) / (blocks * warps);
+  if (have >= 148 * 6 || longest <= 4 * kTileRows) return {q.rows + 1, q.n, false};
+  const long long want = (148 * 12 + blocks * warps - 1) / (blocks * warps);
   long long rows = (q.rows + want - 1) / want;
   rows = (rows + kTileRows - 1) / kTileRows * kTileRows;
   if (rows < 2 * kTileRows) rows = 2 * kTileRows;
