@@ -15,9 +15,12 @@
 // takes W consecutive bytes (2 W values of k) of its two rows and the same
 // values of k of its input row; four lanes make a k block of 8 W values. W is
 // the widest of 16, 8 and 4 with blocks that a group's scale covers whole.
-// A CTA owns 16 R rows and all of k; its eight warps take every eighth k block,
-// with up to U blocks of weights on their way at once, and join through shared
-// memory in a fixed order.
+// A CTA owns 16 R rows and all of k; its NW warps take every NW-th k block and
+// join through shared memory in a fixed order. Many warps with short loops hide
+// more than few with long ones: U blocks of weights and one of inputs are on
+// their way to a warp (four times the weights: 1 x 4096 x 2048 4.9 us, not 4.2).
+// Clusters that shared k and kept the inputs in shared memory took longer (7.0
+// us): the exchange costs more than the reads it saves.
 #include "fav_ops.cuh"
 
 namespace fav {
@@ -30,11 +33,8 @@ struct Int4Args {
   const uint8_t* weight;
   const float *scales, *bias;
   int rows, depth, out, group, groups;
-  int wide;  // input rows start on 16-byte boundaries
 };
 
-constexpr int kInt4Warps = 8;
-constexpr int kInt4Threads = 32 * kInt4Warps;
 
 // The MMA's operand type for inputs of type T, and the parts of an input.
 template <typename T>
@@ -74,43 +74,54 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t word, int j, __nv_bfloat1
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Eight inputs as the four pairs (0,4), (1,5), (2,6), (3,7) of each part.
+// Eight consecutive inputs, and the words that the MMAs take of them: the pairs
+// (0,4), (1,5), (2,6), (3,7) of each part.
 template <typename T>
-__device__ __forceinline__ void input_pairs(const T* p, bool wide, uint32_t (&b)[1][4]) {
-  uint32_t w[4];
-  if (wide) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+struct Inputs {
+  uint32_t w[4 * sizeof(T) / 2];
+};
+template <bool WIDE, typename T>
+__device__ __forceinline__ Inputs<T> load_inputs(const T* p, bool in) {
+  constexpr int N = 4 * sizeof(T) / 2;
+  Inputs<T> v;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+      v.w[i] = q.x, v.w[i + 1] = q.y, v.w[i + 2] = q.z, v.w[i + 3] = q.w;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v.w[i] = __float_as_uint(__ldg(p + i));
   } else {
     const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+    for (int i = 0; i < N; ++i) v.w[i] = __ldg(h + 2 * i) | ((uint32_t)__ldg(h + 2 * i + 1) << 16);
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.w[i] = in ? v.w[i] : 0u;
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void input_pairs(const Inputs<T>& v, uint32_t (&b)[1][4]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    b[0][2 * i] = __byte_perm(w[i], w[i + 2], 0x5410);
-    b[0][2 * i + 1] = __byte_perm(w[i], w[i + 2], 0x7632);
+    b[0][2 * i] = __byte_perm(v.w[i], v.w[i + 2], 0x5410);
+    b[0][2 * i + 1] = __byte_perm(v.w[i], v.w[i + 2], 0x7632);
   }
 }
-__device__ __forceinline__ void input_pairs(const float* p, bool wide, uint32_t (&b)[3][4]) {
-  float v[8];
-  if (wide) {
-    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p[i];
-  }
+__device__ __forceinline__ void input_pairs(const Inputs<float>& v, uint32_t (&b)[3][4]) {
   uint32_t part[3][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     // Truncation, so that the largest values do not round to infinity; what is
     // not finite stays in the first part alone (with a NaN's leading bit).
-    const uint32_t bits = __float_as_uint(v[i]);
+    const uint32_t bits = v.w[i];
     const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
     const bool nan = !finite && (bits & 0x007fffffu);
     part[0][i] = (bits & 0xffff0000u) | (nan ? 0x00400000u : 0u);
-    const float mid = v[i] - __uint_as_float(bits & 0xffff0000u);
+    const float mid = __uint_as_float(bits) - __uint_as_float(bits & 0xffff0000u);
     part[1][i] = finite ? __float_as_uint(mid) & 0xffff0000u : 0u;
     part[2][i] = finite ? __float_as_uint(mid - __uint_as_float(part[1][i])) : 0u;
   }
@@ -141,12 +152,13 @@ __device__ __forceinline__ Codes<W> load_codes(const uint8_t* p) {
 }
 
 // R: tiles of 16 weight rows a warp; C: tiles of 8 input rows.
-template <typename T, int W, int R, int C>
-__global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constant__ Int4Args a) {
+template <typename T, bool WIDE, int W, int R, int C, int NW>
+__global__ void __launch_bounds__(32 * NW) int4_kernel(const __grid_constant__ Int4Args a) {
   using M = typename Int4Type<T>::M;
-  constexpr int P = Int4Type<T>::kParts, KB = 8 * W, U = 64 / (W * R);
+  constexpr int P = Int4Type<T>::kParts, KB = 8 * W, U = 16 / W;
   constexpr int kOut = 16 * R, kIn = 8 * C;
-  __shared__ float s_sum[kInt4Warps][kIn][kOut + 1];
+  extern __shared__ float s_dyn[];
+  float (*s_sum)[kIn][kOut + 1] = reinterpret_cast<float (*)[kIn][kOut + 1]>(s_dyn);
   grid_dependency_sync();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int r0 = blockIdx.x * kOut, m0 = blockIdx.y * kIn;
@@ -162,13 +174,17 @@ __global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constan
       wrow[r][h] = a.weight + row * pitch + t * W;
       srow[r][h] = a.scales + (size_t)row * a.groups;
     }
+  const T* xrow[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c)  // rows behind the last repeat it: their sums are not stored
+    xrow[c] = static_cast<const T*>(a.x) + min(m0 + 8 * c + g, a.rows - 1) * a.x_stride;
   float sum[R][C][4] = {};
-  for (int b0 = warp; b0 < blocks; b0 += kInt4Warps * U) {
+  for (int b0 = warp; b0 < blocks; b0 += NW * U) {
     Codes<W> code[U][R][2];
     float scale[U][R][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int blk = b0 + u * kInt4Warps;
+      const int blk = b0 + u * NW;
       const bool in = blk * KB + t * 2 * W < a.depth;
 #pragma unroll
       for (int r = 0; r < R; ++r)
@@ -178,11 +194,30 @@ __global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constan
           scale[u][r][h] = blk < blocks ? __ldg(srow[r][h] + blk * KB / a.group) : 0.f;
         }
     }
+    // The inputs of a block are read while the one before it is worked on; k
+    // behind the last reads as zero.
+    Inputs<T> next[W / 4][C];
+    const auto fetch = [&](int blk) {
+      const int k = blk * KB + t * 2 * W;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const bool in = k + 8 * i < a.depth;
+          next[i][c] = load_inputs<WIDE>(xrow[c] + (in ? k + 8 * i : 0), in);
+        }
+    };
+    fetch(b0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int blk = b0 + u * kInt4Warps;
+      const int blk = b0 + u * NW;
       if (blk >= blocks) break;
-      const int k = blk * KB + t * 2 * W;
+      Inputs<T> now[W / 4][C];
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) now[i][c] = next[i][c];
+      if (u + 1 < U) fetch(blk + NW);
       float part[R][C][4] = {};
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
@@ -196,10 +231,8 @@ __global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constan
           }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const int m = m0 + 8 * c + g;
-          uint32_t in[P][4] = {};
-          if (m < a.rows && k + 8 * i < a.depth)
-            input_pairs(static_cast<const T*>(a.x) + m * a.x_stride + k + 8 * i, a.wide != 0, in);
+          uint32_t in[P][4];
+          input_pairs(now[i][c], in);
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -225,51 +258,64 @@ __global__ void __launch_bounds__(kInt4Threads) int4_kernel(const __grid_constan
 #pragma unroll
       for (int e = 0; e < 4; ++e) s_sum[warp][8 * c + 2 * t + e % 2][16 * r + 8 * (e / 2) + g] = sum[r][c][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < kIn * kOut; i += kInt4Threads) {
+  for (int i = threadIdx.x; i < kIn * kOut; i += 32 * NW) {
     const int c = i / kOut, r = i % kOut, m = m0 + c, row = r0 + r;
     if (m >= a.rows || row >= a.out) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kInt4Warps; ++w) v += s_sum[w][c][r];
+    for (int w = 0; w < NW; ++w) v += s_sum[w][c][r];
     static_cast<T*>(a.y)[m * a.y_stride + row] = from_f32<T>(a.bias ? v + __ldg(a.bias + row) : v);
   }
 }
 
-template <typename T, int W, int R, int C>
+template <typename T, bool WIDE, int W, int R, int C, int NW>
 cudaError_t launch_tile(const Int4Args& a, cudaStream_t stream) {
   const long long across = ((long long)a.rows + 8 * C - 1) / (8 * C);
   if (across > 65535) return cudaErrorInvalidValue;
-  return launch_op(int4_kernel<T, W, R, C>, dim3((a.out + 16 * R - 1) / (16 * R), (unsigned)across), kInt4Threads, 0,
+  const size_t smem = (size_t)NW * 8 * C * (16 * R + 1) * sizeof(float);
+  if (smem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(int4_kernel<T, WIDE, W, R, C, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_op(int4_kernel<T, WIDE, W, R, C, NW>, dim3((a.out + 16 * R - 1) / (16 * R), (unsigned)across), 32 * NW, smem,
                    stream, a);
 }
 
-template <typename T, int W>
+template <typename T, bool WIDE, int W>
 cudaError_t launch_width(const Int4Args& a, cudaStream_t stream) {
-  // 32 weight rows a CTA where that still gives every SM one: the inputs are
-  // then read and arranged half as often. Up to 32 input rows share a pass
-  // over the weights.
-  if (a.rows <= 8) return a.out >= 148 * 32 ? launch_tile<T, W, 2, 1>(a, stream) : launch_tile<T, W, 1, 1>(a, stream);
-  if (a.rows <= 16) return launch_tile<T, W, 1, 2>(a, stream);
-  return launch_tile<T, W, 1, 4>(a, stream);
+  // Up to 32 input rows share a pass over the weights. More weight rows a CTA
+  // where that still gives every SM one: the inputs are then read and arranged
+  // less often (16 inputs of 8192 x 4096: 16 rows 16 us, 32 rows 12.5, 64 rows in
+  // the registers of eight warps 10.9).
+  const bool many = a.out >= 148 * 32;
+  if (a.rows <= 8) return many ? launch_tile<T, WIDE, W, 2, 1, 16>(a, stream) : launch_tile<T, WIDE, W, 1, 1, 16>(a, stream);
+  if (a.rows <= 16) return many ? launch_tile<T, WIDE, W, 4, 2, 8>(a, stream) : launch_tile<T, WIDE, W, 2, 2, 16>(a, stream);
+  return launch_tile<T, WIDE, W, 2, 4, 16>(a, stream);
+}
+
+template <typename T, bool WIDE>
+cudaError_t launch_group(const Int4Args& a, cudaStream_t stream) {
+  if (a.group % 128 == 0) return launch_width<T, WIDE, 16>(a, stream);
+  if (a.group % 64 == 0) return launch_width<T, WIDE, 8>(a, stream);
+  return launch_width<T, WIDE, 4>(a, stream);
 }
 
 template <typename T>
-cudaError_t launch_group(const Int4Args& a, cudaStream_t stream) {
-  if (a.group % 128 == 0) return launch_width<T, 16>(a, stream);
-  if (a.group % 64 == 0) return launch_width<T, 8>(a, stream);
-  return launch_width<T, 4>(a, stream);
+cudaError_t launch_type(const Int4Args& a, bool wide, cudaStream_t stream) {
+  return wide ? launch_group<T, true>(a, stream) : launch_group<T, false>(a, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_project_int4(const fav_int4_args& c, cudaStream_t stream) {
-  Int4Args a{c.x, c.y, c.x_stride, c.y_stride, c.weight, c.scales, c.bias, c.rows, c.depth, c.out, c.group,
-             (c.depth + c.group - 1) / c.group, 0};
+  const Int4Args a{c.x, c.y, c.x_stride, c.y_stride, c.weight, c.scales, c.bias, c.rows, c.depth, c.out, c.group,
+             (c.depth + c.group - 1) / c.group};
   const int elem = elem_bytes(c.type);
-  a.wide = aligned_for(c.x, c.x_stride, elem, 16 / elem);
-  if (c.type == FAV_TYPE_F32) return launch_group<float>(a, stream);
-  if (c.type == FAV_TYPE_BF16) return launch_group<__nv_bfloat16>(a, stream);
-  return launch_group<__half>(a, stream);
+  const bool wide = aligned_for(c.x, c.x_stride, elem, 16 / elem);
+  if (c.type == FAV_TYPE_F32) return launch_type<float>(a, wide, stream);
+  if (c.type == FAV_TYPE_BF16) return launch_type<__nv_bfloat16>(a, wide, stream);
+  return launch_type<__half>(a, wide, stream);
 }
 
 }  // namespace fav
