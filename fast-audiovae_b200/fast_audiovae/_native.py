@@ -91,6 +91,11 @@ SIGNATURES = {
     "fav_selective_scan_workspace_bytes": ([_P], ct.c_size_t),
     "fav_group_norm": ([_P, _P], ct.c_int32),
     "fav_project_int4": ([_P, _P], ct.c_int32),
+    "fav_bind_tensors": ([_P, _P], ct.c_int32),
+    "fav_causal_conv_tensors": ([ct.py_object] * 8 + [ct.c_int32], ct.c_int32),
+    "fav_scan_step_tensors": ([ct.py_object] * 12 + [ct.c_int32], ct.c_int32),
+    "fav_norm_rows_tensors": ([ct.py_object] * 6 + [ct.c_int32, ct.c_float, ct.c_int32], ct.c_int32),
+    "fav_project_int4_tensors": ([ct.py_object] * 5 + [ct.c_int32], ct.c_int32),
     "fav_test_gemm": ([_P, ct.c_int32, ct.c_int32, _P, ct.c_int32, ct.c_int32, _P, _P], ct.c_int32),
     "fav_test_sine": ([_P, ct.c_int32, _P, _P], ct.c_int32),
 }
@@ -124,6 +129,24 @@ def load_library(path=None):
         if path is None:
             _lib = lib
         return lib
+
+
+def tensor_functions(tensor_type):
+    """The entry points that read tensor objects themselves, as functions that keep the interpreter's
+    lock; None when ``tensor_type`` has no DLPack 1.x C exchange interface."""
+    lib = load_library()
+    capsule = getattr(tensor_type, "__dlpack_c_exchange_api__", None)
+    if capsule is None:
+        return None
+    pointer = ct.PYFUNCTYPE(ct.c_void_p, ct.py_object, ct.c_char_p)(("PyCapsule_GetPointer", ct.pythonapi))
+    if lib.fav_bind_tensors(pointer(capsule, b"dlpack_exchange_api"), id(None)) != 0:
+        return None
+    held = ct.PyDLL(str(LIBRARY))
+    for name in ("fav_causal_conv_tensors", "fav_scan_step_tensors", "fav_norm_rows_tensors",
+                 "fav_project_int4_tensors"):
+        fn = getattr(held, name)
+        fn.argtypes, fn.restype = SIGNATURES[name]
+    return held
 
 
 def check(lib, status):

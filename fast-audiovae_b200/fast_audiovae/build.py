@@ -18,7 +18,7 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIBRARY = PACKAGE_DIR / "libfav_cuda.so"
 SOURCES = ("fav_kernels.cu", "fav_tail.cu", "fav_stage.cu", "fav_prepass.cu", "fav_api.cu", "fav_conv.cu", "fav_scan.cu",
-           "fav_norm.cu", "fav_int4.cu", "fav_ops_api.cu")
+           "fav_norm.cu", "fav_int4.cu", "fav_ops_api.cu", "fav_tensors.cu")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "--threads", "0", "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 

@@ -53,9 +53,32 @@ _I32, _F32 = torch.int32, torch.float32
 _FRESH = 2
 _lib = None
 _grad_enabled = torch.is_grad_enabled
-_current_device = torch.cuda.current_device
+_empty_like = torch.empty_like
+# A CUDA tensor in hand means that CUDA is initialised: its own getters will do.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+# A step's call must not cost more than its kernel, so plain tensors go to entry
+# points that read and check them natively (a fifth of the time that it takes from
+# here). What those do not take is checked below, which also says what is wrong.
+_KINDS = {torch.Tensor, torch.nn.Parameter, type(None)}
+_held = False  # not looked for yet; None where the tensors cannot be read natively
+
+
+def _native_path(*tensors):
+    """The native entry points, if all of ``tensors`` are plain ones without gradients."""
+    global _held
+    if _held is False:
+        _held = _native.tensor_functions(torch.Tensor) if torch.cuda.is_available() else None
+    if _held is None or not _KINDS.issuperset(map(type, tensors)):
+        return None
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return None
+    return _held
 
 
 def _library(index):
@@ -89,11 +112,8 @@ def _main(x):
         raise ValueError("x must be a float32, bfloat16 or float16 tensor") from None
 
 
-def _graph_free(*tensors):
-    if _grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("Stream operators have no gradients; call them under torch.no_grad()")
+def _no_gradients():
+    raise RuntimeError("Stream operators have no gradients; call them under torch.no_grad()")
 
 
 def _array(t, name, dtype, index, shape):
@@ -187,8 +207,13 @@ def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=No
     sequence's first come from ``state`` ``[slots, 2, taps - 1, channels]`` (x's
     type, oldest first; ``conv_state`` makes one) or are zero.
     """
+    native = _native_path(x, weight, bias, offsets, state, codes, status, out)
+    if native is not None and (activation is None or activation == "silu"):
+        y = _empty_like(x) if out is None else out
+        if native.fav_causal_conv_tensors(x, weight, bias, offsets, state, codes, status, y,
+                                          _ACTIVATIONS[activation]) == 0:
+            return y
     kind, index = _main(x)
-    _graph_free(x, weight, bias)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
@@ -202,10 +227,14 @@ def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=No
     x_at, x_stride = _array(x, "x", dtype, index, shape)
     pool_at, codes_at, slots = _states(state, codes, dtype, index, n, (2, taps - 1, channels))
     status_at = _index(status, "status", index, 1) if status is not None else 0
+    if _grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        _no_gradients()
     lib = _library(index)
-    if out is None:
-        out = torch.empty_like(x)
-    y_at, y_stride = _array(out, "out", dtype, index, shape)
+    if out is None:  # contiguous: x's rows have one stride, or lie that way themselves
+        out = _empty_like(x)
+        y_at, y_stride = out.data_ptr(), channels
+    else:
+        y_at, y_stride = _array(out, "out", dtype, index, shape)
     if n:
         _call(lib, lib.fav_causal_conv,
               CONV_ARGS(x_at, y_at, x_stride, y_stride, weight_at, bias_at, pool_at, codes_at, offsets_at, status_at,
@@ -244,8 +273,13 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
     is ``[N, channels]`` and ``d`` and ``dt_bias`` are ``[channels]``. N is 1 to
     128. ``state`` is ``[slots, 2, N, channels]`` fp32 (``scan_state``).
     """
+    if offsets is None:
+        native = _native_path(x, dt, a, b, c, d, z, dt_bias, state, codes, status, out)
+        if native is not None:
+            y = _empty_like(x) if out is None else out
+            if native.fav_scan_step_tensors(x, dt, a, b, c, d, z, dt_bias, state, codes, status, y, bool(softplus)) == 0:
+                return y
     kind, index = _main(x)
-    _graph_free(x, dt, a, b, c, d, z, dt_bias)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
@@ -266,10 +300,16 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
     bias_at = _vector(dt_bias, "dt_bias", index, (channels,))
     pool_at, codes_at, slots = _states(state, codes, _F32, index, n, (2, states, channels))
     status_at = _index(status, "status", index, 1) if status is not None else 0
+    if _grad_enabled() and (x.requires_grad or dt.requires_grad or a.requires_grad or b.requires_grad or c.requires_grad or
+                            (d is not None and d.requires_grad) or (z is not None and z.requires_grad) or
+                            (dt_bias is not None and dt_bias.requires_grad)):
+        _no_gradients()
     lib = _library(index)
-    if out is None:
-        out = torch.empty_like(x)
-    y_at, y_stride = _array(out, "out", dtype, index, shape)
+    if out is None:  # contiguous: x's rows have one stride, or lie that way themselves
+        out = _empty_like(x)
+        y_at, y_stride = out.data_ptr(), channels
+    else:
+        y_at, y_stride = _array(out, "out", dtype, index, shape)
     if not n:
         return out
     fixed = (x_at, dt_at, z_at, b_at, c_at, y_at, x_stride, dt_stride, z_stride, b_stride, b_group, c_stride, c_group,
@@ -296,8 +336,14 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     ``activation`` is None, ``"silu"`` or ``"snake"``, the decoder's
     ``v + reciprocal * sin(alpha * v)**2`` with ``[channels]`` coefficients.
     """
+    if offsets is None and status is None and type(groups) is int and activation in _ACTIVATIONS and eps >= 0:
+        native = _native_path(x, weight, bias, alpha, reciprocal, out)
+        if native is not None:
+            y = _empty_like(x) if out is None else out
+            if native.fav_norm_rows_tensors(x, weight, bias, alpha, reciprocal, y, groups, eps,
+                                            _ACTIVATIONS[activation]) == 0:
+                return y
     kind, index = _main(x)
-    _graph_free(x, weight, bias, alpha, reciprocal)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
@@ -314,10 +360,16 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
                     _vector(alpha, "alpha", index, per), _vector(reciprocal, "reciprocal", index, per))
     x_at, x_stride = _array(x, "x", dtype, index, shape)
     status_at = _index(status, "status", index, 1) if status is not None else 0
+    if _grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                            (bias is not None and bias.requires_grad) or
+                            (alpha is not None and (alpha.requires_grad or reciprocal.requires_grad))):
+        _no_gradients()
     lib = _library(index)
-    if out is None:
-        out = torch.empty_like(x)
-    y_at, y_stride = _array(out, "out", dtype, index, shape)
+    if out is None:  # contiguous: x's rows have one stride, or lie that way themselves
+        out = _empty_like(x)
+        y_at, y_stride = out.data_ptr(), channels
+    else:
+        y_at, y_stride = _array(out, "out", dtype, index, shape)
     if n:
         _call(lib, lib.fav_group_norm,
               NORM_ARGS(x_at, y_at, x_stride, y_stride, *coefficients, offsets_at, status_at, eps, kind, channels,
@@ -334,8 +386,12 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
     (``quantize_int4`` makes both), ``x`` ``[rows, depth]``. ``group`` and the
     depth are multiples of 32.
     """
+    native = _native_path(x, weight, scales, bias, out)
+    if native is not None and type(group) is int and weight is not None and x.dim() == 2 and weight.dim() == 2:
+        y = x.new_empty((x.shape[0], weight.shape[0])) if out is None else out
+        if native.fav_project_int4_tensors(x, weight, scales, bias, y, group) == 0:
+            return y
     kind, index = _main(x)
-    _graph_free(x, scales, bias)
     shape, dtype = x.shape, x.dtype
     if len(shape) != 2:
         raise ValueError("x must have shape [rows, depth]")
@@ -359,10 +415,14 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
     scales_at = _vector(scales, "scales", index, (width, -(-depth // group)))
     bias_at = _vector(bias, "bias", index, (width,))
     x_at, x_stride = _array(x, "x", dtype, index, shape)
+    if _grad_enabled() and (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)):
+        _no_gradients()
     lib = _library(index)
     if out is None:
         out = x.new_empty((rows, width))
-    y_at, y_stride = _array(out, "out", dtype, index, (rows, width))
+        y_at, y_stride = out.data_ptr(), width
+    else:
+        y_at, y_stride = _array(out, "out", dtype, index, (rows, width))
     if rows and width:
         _call(lib, lib.fav_project_int4,
               INT4_ARGS(x_at, y_at, x_stride, y_stride, weight_at, scales_at, bias_at, kind, rows, depth, width, group),

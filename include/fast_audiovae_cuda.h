@@ -366,6 +366,24 @@ typedef struct fav_int4_args {
 } fav_int4_args;
 FAV_API int32_t fav_project_int4(const fav_int4_args *args, void *cuda_stream);
 
+/* The operators on Python tensor objects, for a binding that calls with the
+ * interpreter's lock held and has seen that each object is a tensor of the
+ * framework whose DLPack C exchange interface (DLPack 1.x,
+ * `dlpack_exchange_api`) was bound, or None (`none`) for an absent one. They read
+ * the tensors, check them as the functions above need them and launch on the
+ * current stream of x's device. They return an fav_status, or -1 when a tensor
+ * is not what the operator takes, or not on the current device: the binding then
+ * checks for itself and says so. fav_scan_step_tensors and fav_norm_rows_tensors
+ * take single rows ([rows][channels]) alone, which need no workspace. */
+FAV_API int32_t fav_bind_tensors(const void *exchange, void *none);
+FAV_API int32_t fav_causal_conv_tensors(void *x, void *weight, void *bias, void *offsets, void *state, void *codes,
+                                        void *status, void *y, int32_t activation);
+FAV_API int32_t fav_scan_step_tensors(void *x, void *dt, void *a, void *b, void *c, void *d, void *z, void *dt_bias,
+                                      void *state, void *codes, void *status, void *y, int32_t softplus);
+FAV_API int32_t fav_norm_rows_tensors(void *x, void *weight, void *bias, void *alpha, void *reciprocal, void *y,
+                                      int32_t groups, float eps, int32_t activation);
+FAV_API int32_t fav_project_int4_tensors(void *x, void *weight, void *scales, void *bias, void *y, int32_t group);
+
 #ifdef __cplusplus
 }
 #endif
