@@ -221,14 +221,15 @@ __global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(cons
       for (int u = 0; u < U; ++u) win[H + u] = widen(ring[(at + u) * kConvThreads]);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        if (live) store_pack<T, V>(py, narrow<T, V>(th.row(win + u)));
+        py += a.y_stride;
+      }
+      // Into the places just read: after the stores, which have waited for the reads.
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
         if (r + D + u < last) copy_pack<T, V>(ring + (at + u) * kConvThreads, px);
         copy_commit();
         px += a.x_stride;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (live) store_pack<T, V>(py, narrow<T, V>(th.row(win + u)));
-        py += a.y_stride;
       }
 #pragma unroll
       for (int j = 0; j < H; ++j) win[j] = win[j + U];
@@ -236,11 +237,11 @@ __global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(cons
     } else {
       copy_wait<D - 1>();
       win[H] = widen(ring[at * kConvThreads]);
+      if (live) store_pack<T, V>(py, narrow<T, V>(th.row(win)));
+      py += a.y_stride;
       if (r + D < last) copy_pack<T, V>(ring + at * kConvThreads, px);
       copy_commit();
       px += a.x_stride;
-      if (live) store_pack<T, V>(py, narrow<T, V>(th.row(win)));
-      py += a.y_stride;
 #pragma unroll
       for (int j = 0; j < H; ++j) win[j] = win[j + 1];
       ++r;

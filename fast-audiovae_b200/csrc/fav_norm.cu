@@ -258,9 +258,6 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
   return {n, fmaf(d, f, a.mean), a.squares + b.squares + d * d * a.count * f};
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 template <typename T, int V, int NT>
 __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(const __grid_constant__ NormArgs a) {
   extern __shared__ __align__(16) unsigned char s_raw[];
@@ -409,7 +406,7 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
     s_mean[g] = all.mean;
     s_rstd[g] = all.count > 0.f ? rsqrtf(all.squares / all.count + a.eps) : 0.f;
   }
-  if (ctas > 1) cluster_arrive();  // done with the others' statistics
+  if (ctas > 1) cluster.barrier_arrive();  // done with the others' statistics
   __syncthreads();
   if (dv == 0) {
     // One vector of channels for good: its coefficients stay in registers.
@@ -437,7 +434,7 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
       if (v >= vecs) ++r, v -= vecs;
     }
   }
-  if (ctas > 1) cluster_wait();  // no CTA leaves while another reads its statistics
+  if (ctas > 1) cluster.barrier_wait();  // no CTA leaves while another reads its statistics
 }
 
 constexpr int kMaxNormSmem = 200 * 1024;

@@ -55,9 +55,10 @@ bool overlap(const View& a, const View& b) {
 }
 
 int32_t check_stride(const char* name, int64_t stride, int32_t width, int32_t rows) {
-  // Rows may not overlap; the last byte must stay within 2^62.
-  if (rows > 1 && (stride < width || stride > (1LL << 30)))
-    return fail(FAV_INVALID_ARGUMENT, "%s row stride %lld outside [%d, 2^30]", name, (long long)stride, width);
+  // Rows may not overlap, and byte offsets must stay far inside 64 bits.
+  if (rows > 1 && (stride < width || stride > (1LL << 30) || rows * stride > (1LL << 56)))
+    return fail(FAV_INVALID_ARGUMENT, "%s row stride %lld outside [%d, 2^30], or array too large", name,
+                (long long)stride, width);
   return FAV_OK;
 }
 

@@ -270,7 +270,7 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
 
     ``dt`` and ``z`` are shaped like ``x``; ``b`` and ``c`` are
     ``[..., groups, N]`` over the same rows (groups divide the channels); ``a``
-    is ``[N, channels]`` and ``d`` and ``dt_bias`` are ``[channels]``. N is 1 to
+    is ``[N, channels]`` and finite, and ``d`` and ``dt_bias`` are ``[channels]``. N is 1 to
     128. ``state`` is ``[slots, 2, N, channels]`` fp32 (``scan_state``).
     """
     if offsets is None:

@@ -564,6 +564,134 @@ def test_two_streams_at_once():
             assert torch.equal(y, alone[i])
 
 
+def test_both_ways_of_reading_tensors_agree(monkeypatch):
+    """Plain tensors read natively, and tensors of another class read from Python: the same bits."""
+    class Other(torch.Tensor):
+        pass
+
+    g = gen(8)
+    x, q = normal(g, 6, 64, dtype=BF16).cuda(), torch.randint(0, 256, (48, 32), generator=g, dtype=torch.uint8).cuda()
+    w, b = normal(g, 64, 4).cuda(), normal(g, 64).cuda()
+    maps, a = normal(g, 6, 2, 8, dtype=BF16).cuda(), -torch.rand(8, 64, generator=g).cuda()
+    codes = codes_for(g, 6, 6).cuda()
+    def run(kind):
+        history, state = torch.ones(6, 2, 3, 64, dtype=BF16, device="cuda"), torch.ones(6, 2, 8, 64, device="cuda")
+        first = x.as_subclass(Other) if kind == "subclass" else x
+        return [ops.causal_conv(first, w, b, activation="silu", state=history, codes=codes), history,
+                ops.causal_conv(first.view(2, 3, 64), w),
+                ops.selective_scan(first, x, a, maps, maps, d=b, z=x, dt_bias=b, state=state, codes=codes), state,
+                ops.group_norm(first, 8, b, b, activation="snake", alpha=b, reciprocal=b),
+                ops.project_int4(first, q, torch.ones(48, 2, device="cuda"), w[:48, 0].contiguous(), group=32)]
+    native = run("plain")
+    assert ops._held, "tensors are not read natively here"
+    other = run("subclass")
+    monkeypatch.setattr(ops, "_held", None)
+    python = run("plain")
+    for n, o, p in zip(native, other, python):
+        assert torch.equal(n, o.as_subclass(torch.Tensor)) and torch.equal(n, p)
+
+
+def test_refusals_of_device_tensors():
+    """What the native reading leaves alone is refused with the reason, and nothing is launched."""
+    x, w = torch.zeros(4, 64, device="cuda"), torch.zeros(64, 4, device="cuda")
+    q, s = torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.zeros(8, 2, device="cuda")
+    maps, a = torch.zeros(4, 1, 8, device="cuda"), torch.zeros(8, 64, device="cuda")
+    for call, words in [
+            (lambda: ops.causal_conv(x, w.cpu()), "weight must be"), (lambda: ops.causal_conv(x.cpu(), w), "weight must be"),
+            (lambda: ops.causal_conv(x.double(), w), "x must be"), (lambda: ops.causal_conv(x[:, ::2], w[:32]), "adjacent"),
+            (lambda: ops.causal_conv(x, w.t().contiguous().t()), "weight must be"),
+            (lambda: ops.causal_conv(x, w, activation="snake"), "activation"),
+            (lambda: ops.causal_conv(x, w, out=torch.zeros(4, 64, device="cuda", dtype=F16)), "out must be"),
+            (lambda: ops.causal_conv(x, w, out=torch.zeros(4, 64)), "out must be"),
+            (lambda: ops.selective_scan(x, x.half(), a, maps, maps), "dt must be"),
+            (lambda: ops.selective_scan(x, x, a, maps, maps.cpu()), "c must be"),
+            (lambda: ops.selective_scan(x, x, a[:, :32], maps, maps), "a must be"),
+            (lambda: ops.group_norm(x, 3), "divides"), (lambda: ops.group_norm(x, 4, eps=float("nan")), "eps"),
+            (lambda: ops.group_norm(x, 4, w[:, 0]), "weight must be"),
+            (lambda: ops.project_int4(x, q, s, group=64), "scales must be"),
+            (lambda: ops.project_int4(x, q.char(), s, group=32), "weight must be"),
+            (lambda: ops.project_int4(x, q, s, s[:, 0], group=32), "bias must be")]:
+        with pytest.raises(ValueError, match=words):
+            call()
+    grad = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.group_norm(grad, 4)
+    with torch.no_grad():
+        assert torch.equal(ops.group_norm(grad, 4), x)
+    with pytest.raises(_native.NativeError):   # rows that share memory
+        ops.causal_conv(x[:1].expand(4, 64), w)
+
+
+def test_a_parameter_is_a_tensor():
+    x = torch.ones(3, 64, device="cuda")
+    w = torch.nn.Parameter(torch.ones(64, 2, device="cuda"))
+    with torch.inference_mode():
+        assert torch.equal(ops.causal_conv(x.view(1, 3, 64), w)[0, :, 0].cpu(), torch.tensor([1.0, 2.0, 2.0]))
+
+
+def test_calls_follow_the_current_stream():
+    """A call on a side stream waits for that stream's earlier work alone."""
+    g = gen(12)
+    x, w = normal(g, 40, 64).cuda(), normal(g, 64, 4).cuda()
+    want = ops.causal_conv(x.view(1, 40, 64) * 2, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            y = ops.causal_conv(x.view(1, 40, 64) * 2, w)
+    side.synchronize()
+    assert torch.equal(y, want)
+
+
+def test_captured_graphs_keep_their_own_workspaces():
+    """Two captured prompts (split scans and norms, which need workspaces or clusters), replayed in turn."""
+    g = gen(13)
+    inputs = [{k: v.cuda().unflatten(0, (1, 2000)) if k in ("x", "dt", "b", "c", "z") else v.cuda()
+               for k, v in scan_inputs(g, 2000, 64, 16, 1, F32, True).items()} for _ in range(2)]
+    def run(i):
+        y = ops.selective_scan(**inputs[i])
+        return y, ops.group_norm(y, 8, activation="silu")
+    want = [run(i) for i in range(2)]
+    graphs, got = [], []
+    for i in range(2):
+        side, captured = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(captured, stream=side):
+            got.append(run(i))
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append(captured)
+    for _ in range(3):
+        for captured in graphs:
+            captured.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_more_than_two_to_the_31_elements():
+    """The last rows of arrays of 2.4e9 elements are those of a short call."""
+    rows, channels = 1_200_000, 2048
+    x = torch.zeros(rows, channels, dtype=BF16, device="cuda")
+    tail = normal(gen(14), 40, channels, dtype=BF16).cuda()
+    x[-40:] = tail
+    w = normal(gen(15), channels, 4).cuda()
+    y = ops.causal_conv(x.unsqueeze(0), w, activation="silu")[0]
+    assert torch.equal(y[-36:], ops.causal_conv(tail.unsqueeze(0), w, activation="silu")[0, -36:])
+    assert not y[:-40].any()
+    y = ops.group_norm(x, 16, activation="silu", out=y)
+    assert torch.equal(y[-40:], ops.group_norm(tail, 16, activation="silu"))
+    y = ops.group_norm(x, 16, offsets=torch.tensor([rows - 40, rows], dtype=torch.int32, device="cuda"), out=y)
+    want, tol = ref.group_norm(tail.cpu(), 16, None, None, 1e-5, None, None, None, [(0, 40)])
+    close(y[-40:], want, tol)
+    del y
+    maps = torch.ones(rows, 1, 4, dtype=BF16, device="cuda")
+    a = -torch.ones(4, channels, device="cuda")
+    y = ops.selective_scan(x, x, a, maps, maps, offsets=torch.tensor([0, rows - 40, rows], dtype=torch.int32, device="cuda"))
+    short = ops.selective_scan(tail, tail, a, maps[:40], maps[:40],
+                               offsets=torch.tensor([0, 40], dtype=torch.int32, device="cuda"))
+    assert (y[-40:].float() - short.float()).abs().max() <= short.float().abs().max() * 2 ** -7   # pieces end elsewhere
+
+
 def test_argument_structures_are_the_native_ones():
     """A zero-row call of each operator passes its checks through the C ABI."""
     lib = _native.load_library()

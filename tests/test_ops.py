@@ -93,6 +93,11 @@ def test_the_c_abi_refuses_null(lib):
     assert lib.fav_selective_scan_workspace_bytes(None) == 0
 
 
+def test_binding_tensors_needs_an_exchange(lib):
+    assert lib.fav_bind_tensors(None, None) == 1
+    assert lib.fav_bind_tensors(ct.byref((ct.c_uint32 * 32)(2)), id(None)) == 2   # DLPack 2 is not known
+
+
 def test_scan_workspace_grows_only_for_few_long_sequences(lib):
     def need(n, length, channels):
         return lib.fav_selective_scan_workspace_bytes(ct.byref(_native.ScanArgs(
