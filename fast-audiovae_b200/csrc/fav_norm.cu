@@ -227,7 +227,10 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const __grid_con
   }
 }
 
-constexpr int kThreads = 128, kWideThreads = 512;  // of a CTA: its share of the rows small or large
+constexpr int kWideThreads = 512;  // of a CTA with a large share of the rows
+// Of a CTA with a small one: twice as many for fp32 (64 clips of 750 x 512: 256
+// threads 43 us, 128 45 us; bf16 34 and 30).
+constexpr int small_threads(int v) { return v == 4 ? 256 : 128; }
 constexpr int kMaxCtas = 16;  // of a cluster (above 8 where the device can place them)
 
 // --------------------------------------------------------------- sequences
@@ -491,7 +494,7 @@ cudaError_t launch_sequences(NormArgs a, cudaStream_t stream) {
   // Whole groups, 64 bytes of a row where they are narrower: short rows leave
   // a CTA's share small enough for several an SM without a larger cluster.
   a.block_groups = std::max(1, std::min(a.groups, 64 / (int)(a.width * sizeof(T))));
-  while (a.block_groups > 1 && a.block_groups * vecs > kThreads) --a.block_groups;
+  while (a.block_groups > 1 && a.block_groups * vecs > 128) --a.block_groups;
   a.blocks = (a.groups + a.block_groups - 1) / a.block_groups;
   const size_t row = (size_t)a.block_groups * a.width * sizeof(T), stats = a.block_groups * sizeof(Stats) + 16;
   // Shared memory for sequences of up to twice the mean length.
@@ -512,7 +515,7 @@ cudaError_t launch_sequences(NormArgs a, cudaStream_t stream) {
   if (ctas > 8 && !clusters_fit(norm_kernel<T, V, kWideThreads>, ctas, kWideThreads, smem)) ctas = 8, smem = fit();
   // Large shares, one CTA an SM, need its threads; small ones more CTAs.
   if (smem > 64 * 1024 || ctas > 8) return launch_cluster<T, V, kWideThreads>(a, ctas, smem, stream);
-  return launch_cluster<T, V, kThreads>(a, ctas, smem, stream);
+  return launch_cluster<T, V, small_threads(V)>(a, ctas, smem, stream);
 }
 
 template <typename T, int V>

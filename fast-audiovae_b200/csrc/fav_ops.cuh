@@ -62,6 +62,35 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
   *reinterpret_cast<Pack<T, V>*>(p) = v;
 }
 
+// The same of memory that is not read or written again soon: it leaves the caches
+// first.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_once(const T* p) {
+  constexpr int B = sizeof(T) * V;
+  Pack<T, V> r;
+  if constexpr (B == 16)
+    *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
+  else if constexpr (B == 8)
+    *reinterpret_cast<uint2*>(&r) = __ldcs(reinterpret_cast<const uint2*>(p));
+  else if constexpr (B == 4)
+    *reinterpret_cast<uint32_t*>(&r) = __ldcs(reinterpret_cast<const uint32_t*>(p));
+  else
+    *reinterpret_cast<uint16_t*>(&r) = __ldcs(reinterpret_cast<const uint16_t*>(p));
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_once(T* p, const Pack<T, V>& v) {
+  constexpr int B = sizeof(T) * V;
+  if constexpr (B == 16)
+    __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+  else if constexpr (B == 8)
+    __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(&v));
+  else if constexpr (B == 4)
+    __stcs(reinterpret_cast<uint32_t*>(p), *reinterpret_cast<const uint32_t*>(&v));
+  else
+    __stcs(reinterpret_cast<uint16_t*>(p), *reinterpret_cast<const uint16_t*>(&v));
+}
+
 // A pack from global into shared memory, asynchronously; without an
 // asynchronous copy of that size (2 bytes) at once.
 template <typename T, int V>

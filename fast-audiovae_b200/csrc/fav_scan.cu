@@ -56,8 +56,9 @@ __device__ __forceinline__ float delta_of(const ScanArgs& a, float dt, int c) {
 // bytes a channel), so a thread moves V = 4 neighbouring channels of a state
 // with 16-byte accesses; L lanes of a warp share a channel's states where
 // there are too few channels and streams to fill the GPU. 512 streams of 2048 x 16
-// take 34 us, 60 % of the copy rate. (Holding `a` in registers over several
-// streams took 51 us: the registers cost more warps than the reads of `a` time.)
+// take 27.5 us, 70 % of the copy rate; without the hint that a state is not used
+// again 31. (Holding `a` in registers over several streams took 51 us: the
+// registers cost more warps than the reads of `a` time.)
 constexpr int kStepThreads = 128;
 
 template <typename T, int V, int L>
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
 #pragma unroll
     for (int k = 0; k < B; ++k) {
       const int n = n0 + k * L;
-      h[k] = held && n < a.states ? load_pack<float, V>(from + (size_t)n * a.channels) : Pack<float, V>{};
+      h[k] = held && n < a.states ? load_once<float, V>(from + (size_t)n * a.channels) : Pack<float, V>{};
     }
 #pragma unroll
     for (int k = 0; k < B; ++k) {
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
         h[k].v[i] = fmaf(ex2_approx(scale[i] * av.v[i]), h[k].v[i], dx[i] * bn);
         y[i] = fmaf(h[k].v[i], cn, y[i]);
       }
-      if (keep) store_pack<float, V>(to + (size_t)n * a.channels, h[k]);
+      if (keep) store_once<float, V>(to + (size_t)n * a.channels, h[k]);
     }
   }
 #pragma unroll
