@@ -2,8 +2,11 @@
 //
 //   y[m, r] = bias[r] + sum_g scales[r, g] * sum_{k in g} x[m, k] * (q[r, k] - 8)
 //
-// Bound by reading the weights once (out * depth / 2 bytes). The codes minus 8
-// are exact in fp16 and bf16, so the inner sums run on the tensor cores with
+// The floor is reading the weights once (out * depth / 2 bytes: 2.8 us of 16 x
+// 8192 x 4096, 0.7 us of 1 x 4096 x 2048). They take 10.9 and 4.4 us: the chain of
+// launch, weights, inputs, products and join, a few us long, and for more input
+// rows the reading and arranging of inputs from L1. The codes minus 8 are exact
+// in fp16 and bf16, so the inner sums run on the tensor cores with
 // exact operands: mma.sync m16n8k16, 16 weight rows by 8 input rows, fp32
 // accumulation (an input row or two cannot fill a tcgen05 tile, and the codes
 // must pass the registers anyway to become operands). A block's sum is scaled
@@ -34,7 +37,6 @@ struct Int4Args {
   const float *scales, *bias;
   int rows, depth, out, group, groups;
 };
-
 
 // The MMA's operand type for inputs of type T, and the parts of an input.
 template <typename T>

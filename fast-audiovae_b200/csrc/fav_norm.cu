@@ -9,10 +9,14 @@
 //
 // Bound by memory: x is read once and y written once. Single rows keep a group
 // in the registers of 1 to 256 threads. Longer sequences are cut into blocks of
-// whole groups, about 256 bytes of a row, and a cluster of up to eight CTAs
-// shares a block's rows: each keeps its rows in shared memory, the CTAs exchange
-// their statistics through distributed shared memory, and y is formed from the
-// kept rows. Rows beyond the shared memory are read again (from L2 mostly).
+// whole groups, 64 bytes of a row or one group, and a cluster of up to sixteen
+// CTAs shares a block's rows: each keeps its rows in shared memory, the CTAs
+// exchange their statistics through distributed shared memory, and y is formed
+// from the kept rows. Rows beyond the shared memory are read again (from L2
+// mostly). 64 clips of 750 x 512 fp32 take 43 us, 70 % of the copy rate: a CTA
+// loads, exchanges and stores in turn, so that only several an SM overlap. (Two
+// launches over ranges of rows, which read x twice, took 57 us, and two to four
+// times as long where sequences are short.)
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -138,8 +138,12 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
 // are copied ahead of their use (cp.async) into two buffers, and y takes x's
 // place in them until the tile is stored.
 //
-// Bound by ex2: T * C * N of them at 16 a clock and SM, and four more a value
-// for softplus and gate.
+// Bound by the special function unit: T * C * N times ex2 at 16 a clock and SM,
+// and four more a value for softplus and gate. 32 ragged prompts of up to 750 x
+// 1536 x 16 in fp32 need 100 us of it and take 167: it is busy two thirds of the
+// time on the SMs that have work, and the SMs' shares differ. (A quarter of the
+// powers by a polynomial on the FMA pipe took 10 % longer: the instructions it
+// adds are as scarce.)
 constexpr int kTileRows = 16;
 constexpr int kBlockChannels = 64;
 
@@ -191,9 +195,9 @@ __device__ __forceinline__ Piece piece_at(const ScanArgs& a, int p) {
   return r;
 }
 
-// The sequence that is number `rank` by length, longest first (n <= NT). In that
-// order every SM gets long and short ones alike: 33 prompts of up to 750 rows,
-// all resident at once, took as long as the SM with the most rows.
+// The sequence that is number `rank` by length, longest first (n <= NT): the
+// blocks that start last are then the short ones (33 prompts of up to 750 rows
+// 226 us in their own order, 171 in this one).
 template <int NT>
 __device__ __forceinline__ int sequence_by_length(const Sequences& q, int rank) {
   __shared__ int s_length[NT], s_pick;
@@ -437,10 +441,12 @@ __global__ void __launch_bounds__(kBlockChannels* L, L == 2 ? 3 : 1) scan_kernel
 template <typename T, int V>
 cudaError_t launch_step(const ScanArgs& a, cudaStream_t stream) {
   const long long items = (long long)a.seq.n * (a.channels / V);
-  // Four lanes per channel vector while one would leave an SM under 1024 threads.
-  const int lanes = items < 148 * 1024 ? 4 : 1;
+  // Four lanes per channel vector while one would leave an SM under 1024 threads,
+  // sixteen while four would leave it under 128 (1 x 1024 channels 2.6 us, not 3.1).
+  const int lanes = items >= 148 * 1024 ? 1 : items >= 148 * 32 ? 4 : 16;
   const long long blocks = (items * lanes + kStepThreads - 1) / kStepThreads;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (lanes == 16) return launch_op(scan_step_kernel<T, V, 16>, (unsigned)blocks, kStepThreads, 0, stream, a);
   if (lanes == 4) return launch_op(scan_step_kernel<T, V, 4>, (unsigned)blocks, kStepThreads, 0, stream, a);
   return launch_op(scan_step_kernel<T, V, 1>, (unsigned)blocks, kStepThreads, 0, stream, a);
 }

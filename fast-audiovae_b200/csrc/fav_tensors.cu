@@ -40,8 +40,8 @@ void* g_none = nullptr;
 
 struct Tensor {
   DlTensor t;
-  bool read(void* object) {
-    return g_exchange->view(object, &t) == 0 && t.device_type == kDlCuda && t.strides && t.lanes == 1;
+  bool read(void* object) {  // false of None too, which the exchange must not be given
+    return object != g_none && g_exchange->view(object, &t) == 0 && t.device_type == kDlCuda && t.strides && t.lanes == 1;
   }
   const char* data() const { return static_cast<const char*>(t.data) + t.byte_offset; }
   bool is(uint8_t code, uint8_t bits) const { return t.code == code && t.bits == bits; }

@@ -14,6 +14,10 @@ takes ``weights=`` (a coefficient dict, names from
 ``fast_audiovae.weights.weight_shapes()``), ``source=`` an ``.npz`` file with
 those names, or, by default, the seeded random init of
 ``fast_audiovae.weights.seeded_weights(weight_seed)``.
+
+``fast_audiovae.ops`` (imported on its own) has the operators of a recurrent
+model that makes latents for many streams: causal convolution, selective scan,
+group norm and 4-bit projection on device tensors.
 """
 from __future__ import annotations
 

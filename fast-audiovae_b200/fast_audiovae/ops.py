@@ -68,8 +68,10 @@ _held = False  # not looked for yet; None where the tensors cannot be read nativ
 
 
 def _native_path(*tensors):
-    """The native entry points, if all of ``tensors`` are plain ones without gradients."""
+    """The native entry points, if all of ``tensors`` are plain ones without gradients, or None but for the first."""
     global _held
+    if tensors[0] is None:
+        return None
     if _held is False:
         _held = _native.tensor_functions(torch.Tensor) if torch.cuda.is_available() else None
     if _held is None or not _KINDS.issuperset(map(type, tensors)):

@@ -606,6 +606,14 @@ def test_refusals_of_device_tensors():
             (lambda: ops.selective_scan(x, x.half(), a, maps, maps), "dt must be"),
             (lambda: ops.selective_scan(x, x, a, maps, maps.cpu()), "c must be"),
             (lambda: ops.selective_scan(x, x, a[:, :32], maps, maps), "a must be"),
+            (lambda: ops.causal_conv(None, w), "x must be"), (lambda: ops.causal_conv(x, None), "weight must"),
+            (lambda: ops.selective_scan(x, None, a, maps, maps), "dt must be"),
+            (lambda: ops.selective_scan(x, x, None, maps, maps), "a must have"),
+            (lambda: ops.selective_scan(x, x, a, None, maps), "b must have"),
+            (lambda: ops.selective_scan(x, x, a, maps, None), "c must be"),
+            (lambda: ops.group_norm(None, 4), "x must be"), (lambda: ops.project_int4(None, q, s, group=32), "x must be"),
+            (lambda: ops.project_int4(x, None, s, group=32), "weight must be"),
+            (lambda: ops.project_int4(x, q, None, group=32), "scales are required"),
             (lambda: ops.group_norm(x, 3), "divides"), (lambda: ops.group_norm(x, 4, eps=float("nan")), "eps"),
             (lambda: ops.group_norm(x, 4, w[:, 0]), "weight must be"),
             (lambda: ops.project_int4(x, q, s, group=64), "scales must be"),
