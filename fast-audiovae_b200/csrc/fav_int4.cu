@@ -3,7 +3,7 @@
 //   y[m, r] = bias[r] + sum_g scales[r, g] * sum_{k in g} x[m, k] * (q[r, k] - 8)
 //
 // The floor is reading the weights once (out * depth / 2 bytes: 2.8 us of 16 x
-// 8192 x 4096, 0.7 us of 1 x 4096 x 2048). They take 10.9 and 4.4 us: the chain of
+// 8192 x 4096, 0.7 us of 1 x 4096 x 2048). They take 10.9 and 4.2 us: the chain of
 // launch, weights, inputs, products and join, a few us long, and for more input
 // rows the reading and arranging of inputs from L1. The codes minus 8 are exact
 // in fp16 and bf16, so the inner sums run on the tensor cores with
@@ -20,8 +20,10 @@
 // the widest of 16, 8 and 4 with blocks that a group's scale covers whole.
 // A CTA owns 16 R rows and all of k; its NW warps take every NW-th k block and
 // join through shared memory in a fixed order. Many warps with short loops hide
-// more than few with long ones: U blocks of weights and one of inputs are on
-// their way to a warp (four times the weights: 1 x 4096 x 2048 4.9 us, not 4.2).
+// more than few with long ones: a warp has U blocks of weights and inputs on
+// their way at once, 16 bytes of weights a lane and row. (Twice and four times as
+// much, 1 x 64 x 4096 3.8 and 4.9 us instead of 3.4: straight code that runs once
+// costs more to fetch than the wait it saves.)
 // Clusters that shared k and kept the inputs in shared memory took longer (7.0
 // us): the exchange costs more than the reads it saves.
 #include "fav_ops.cuh"
@@ -196,30 +198,19 @@ __global__ void __launch_bounds__(32 * NW) int4_kernel(const __grid_constant__ I
           scale[u][r][h] = blk < blocks ? __ldg(srow[r][h] + blk * KB / a.group) : 0.f;
         }
     }
-    // The inputs of a block are read while the one before it is worked on; k
-    // behind the last reads as zero.
-    Inputs<T> next[W / 4][C];
-    const auto fetch = [&](int blk) {
-      const int k = blk * KB + t * 2 * W;
+    Inputs<T> in[U][W / 4][C];  // k behind the last reads as zero
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < W / 4; ++i)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const bool in = k + 8 * i < a.depth;
-          next[i][c] = load_inputs<WIDE>(xrow[c] + (in ? k + 8 * i : 0), in);
+          const int k = (b0 + u * NW) * KB + t * 2 * W + 8 * i;
+          in[u][i][c] = load_inputs<WIDE>(xrow[c] + (k < a.depth ? k : 0), k < a.depth);
         }
-    };
-    fetch(b0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int blk = b0 + u * NW;
-      if (blk >= blocks) break;
-      Inputs<T> now[W / 4][C];
-#pragma unroll
-      for (int i = 0; i < W / 4; ++i)
-#pragma unroll
-        for (int c = 0; c < C; ++c) now[i][c] = next[i][c];
-      if (u + 1 < U) fetch(blk + NW);
+      if (b0 + u * NW >= blocks) break;
       float part[R][C][4] = {};
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
@@ -233,14 +224,14 @@ __global__ void __launch_bounds__(32 * NW) int4_kernel(const __grid_constant__ I
           }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          uint32_t in[P][4];
-          input_pairs(now[i][c], in);
+          uint32_t part_in[P][4];
+          input_pairs(in[u][i][c], part_in);
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int q = P - 1; q >= 0; --q) {
-              mma_16816(part[r][c], op[r][0], in[q][0], in[q][1], M{});
-              mma_16816(part[r][c], op[r][1], in[q][2], in[q][3], M{});
+              mma_16816(part[r][c], op[r][0], part_in[q][0], part_in[q][1], M{});
+              mma_16816(part[r][c], op[r][1], part_in[q][2], part_in[q][3], M{});
             }
         }
       }
