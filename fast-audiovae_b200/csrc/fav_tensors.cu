@@ -141,6 +141,43 @@ bool states(void* pool, void* codes, const Tensor& x, uint8_t code, uint8_t bits
   return indices(codes, x, n, codes_at) && *codes_at;
 }
 
+// An input or output map [..., groups, states] over x's rows.
+bool map_of(const Tensor& m, const Tensor& x, const Rows& r, int64_t states, const void** address, int64_t* stride,
+            int64_t* group_stride) {
+  const int lead = x.t.ndim - 1;
+  if (m.t.ndim != lead + 2 || m.t.code != x.t.code || m.t.bits != x.t.bits || m.t.device_id != x.t.device_id) return false;
+  for (int i = 0; i < lead; ++i)
+    if (m.t.shape[i] != x.t.shape[i]) return false;
+  const int64_t groups = m.t.shape[lead];
+  if (groups < 1 || r.channels % groups || m.t.shape[lead + 1] != states || (m.t.strides[lead + 1] != 1 && states != 1))
+    return false;
+  if (lead == 1 || r.length == 1)
+    *stride = m.t.strides[0];
+  else if (r.n == 1 || m.t.strides[0] == r.length * m.t.strides[1])
+    *stride = m.t.strides[1];
+  else
+    return false;
+  if (r.rows == 1) *stride = groups * states;
+  *group_stride = groups > 1 ? m.t.strides[lead] : 0;
+  *address = m.data();
+  return true;
+}
+
+// Sequences of x: packed by `offsets`, or of its shape.
+bool sequences_of(void* offsets, const Tensor& x, const Rows& r, const int32_t** address, int32_t* n, int32_t* length) {
+  *address = nullptr;
+  *n = (int32_t)r.n;
+  *length = (int32_t)r.length;
+  if (offsets == g_none) return true;
+  Tensor o;
+  if (x.t.ndim != 2 || !o.read(offsets) || o.t.ndim != 1 || o.t.shape[0] < 2 || o.t.shape[0] > 0x7fffffff ||
+      !indices(offsets, x, o.t.shape[0], address))
+    return false;
+  *n = (int32_t)o.t.shape[0] - 1;
+  *length = 0;
+  return true;
+}
+
 // The current stream of x's device, which must be the current device.
 bool stream_of(const Tensor& x, void** stream) {
   int device = -1;
@@ -174,17 +211,10 @@ int32_t fav_causal_conv_tensors(void* x, void* weight, void* bias, void* offsets
   if (!xt.read(x) || (a.type = xt.type()) < 0 || !rows_of(xt.t, &r)) return kAsk;
   if (!wt.read(weight) || wt.t.ndim != 2 || wt.t.shape[1] < 2 || wt.t.shape[1] > 8) return kAsk;
   const int64_t taps = wt.t.shape[1];
-  int64_t n = r.n;
-  if (offsets != g_none) {
-    Tensor o;
-    if (xt.t.ndim != 2 || !o.read(offsets) || o.t.ndim != 1 || o.t.shape[0] < 2 || o.t.shape[0] > 0x7fffffff ||
-        !indices(offsets, xt, o.t.shape[0], &a.offsets))
-      return kAsk;
-    n = o.t.shape[0] - 1;
-  }
+  if (!sequences_of(offsets, xt, r, &a.offsets, &a.n, &a.length)) return kAsk;
   void* stream = nullptr;
   if (!coefficients(weight, xt, {r.channels, taps}, &a.weight) || !coefficients(bias, xt, {r.channels}, &a.bias) ||
-      !states(state, codes, xt, xt.t.code, xt.t.bits, n, taps - 1, r.channels, &a.state_pool, &a.slot_codes, &a.num_slots) ||
+      !states(state, codes, xt, xt.t.code, xt.t.bits, a.n, taps - 1, r.channels, &a.state_pool, &a.slot_codes, &a.num_slots) ||
       !indices(status, xt, 1, &a.status) || !same_rows(y, xt, &a.y, &a.y_stride) || !stream_of(xt, &stream))
     return kAsk;
   a.x = xt.data();
@@ -192,65 +222,67 @@ int32_t fav_causal_conv_tensors(void* x, void* weight, void* bias, void* offsets
   a.channels = (int32_t)r.channels;
   a.taps = (int32_t)taps;
   a.activation = activation;
-  a.n = (int32_t)n;
-  a.length = a.offsets ? 0 : (int32_t)r.length;
   a.rows = (int32_t)r.rows;
   return fav_causal_conv(&a, stream);
 }
 
-int32_t fav_scan_step_tensors(void* x, void* dt, void* a_, void* b, void* c, void* d, void* z, void* dt_bias, void* state,
-                              void* codes, void* status, void* y, int32_t softplus) {
+int64_t fav_selective_scan_tensors(void* x, void* dt, void* a_, void* b, void* c, void* d, void* z, void* dt_bias,
+                                   void* offsets, void* state, void* codes, void* status, void* workspace, void* y,
+                                   int32_t softplus) {
   if (!g_exchange) return kAsk;
   Tensor xt, at, bt, ct;
   Rows r;
   fav_scan_args a{};
-  if (!xt.read(x) || (a.type = xt.type()) < 0 || xt.t.ndim != 2 || !rows_of(xt.t, &r)) return kAsk;
+  if (!xt.read(x) || (a.type = xt.type()) < 0 || !rows_of(xt.t, &r)) return kAsk;
   if (!at.read(a_) || at.t.ndim != 2 || at.t.shape[0] < 1 || at.t.shape[0] > 128) return kAsk;
-  const int64_t states_ = at.t.shape[0];
-  if (!bt.read(b) || bt.t.ndim != 3 || bt.t.shape[1] < 1 || r.channels % bt.t.shape[1]) return kAsk;
-  const int64_t groups = bt.t.shape[1];
-  if (!ct.read(c)) return kAsk;
-  for (const Tensor* m : {&bt, &ct})
-    if (m->t.code != xt.t.code || m->t.bits != xt.t.bits || m->t.device_id != xt.t.device_id ||
-        !m->has_shape({r.rows, groups, states_}) || (m->t.strides[2] != 1 && states_ != 1))
-      return kAsk;
+  if (!bt.read(b) || !ct.read(c) || !map_of(bt, xt, r, at.t.shape[0], &a.b, &a.b_stride, &a.b_group_stride) ||
+      !map_of(ct, xt, r, at.t.shape[0], &a.c, &a.c_stride, &a.c_group_stride) ||
+      bt.t.shape[bt.t.ndim - 2] != ct.t.shape[ct.t.ndim - 2])
+    return kAsk;
+  const int64_t states_ = at.t.shape[0], groups = bt.t.shape[bt.t.ndim - 2];
   void* stream = nullptr;
-  if (!coefficients(a_, xt, {states_, r.channels}, &a.a) || !coefficients(d, xt, {r.channels}, &a.d) ||
+  if (!sequences_of(offsets, xt, r, &a.offsets, &a.n, &a.length) ||
+      !coefficients(a_, xt, {states_, r.channels}, &a.a) || !coefficients(d, xt, {r.channels}, &a.d) ||
       !coefficients(dt_bias, xt, {r.channels}, &a.dt_bias) || !same_rows(dt, xt, &a.dt, &a.dt_stride) ||
       (z != g_none && !same_rows(z, xt, &a.z, &a.z_stride)) ||
-      !states(state, codes, xt, kDlFloat, 32, r.n, states_, r.channels, &a.state_pool, &a.slot_codes, &a.num_slots) ||
+      !states(state, codes, xt, kDlFloat, 32, a.n, states_, r.channels, &a.state_pool, &a.slot_codes, &a.num_slots) ||
       !indices(status, xt, 1, &a.status) || !same_rows(y, xt, &a.y, &a.y_stride) || !stream_of(xt, &stream))
     return kAsk;
   a.x = xt.data();
   a.x_stride = r.stride;
-  a.b = bt.data();
-  a.c = ct.data();
-  a.b_stride = r.rows > 1 ? bt.t.strides[0] : groups * states_;
-  a.c_stride = r.rows > 1 ? ct.t.strides[0] : groups * states_;
-  a.b_group_stride = groups > 1 ? bt.t.strides[1] : 0;
-  a.c_group_stride = groups > 1 ? ct.t.strides[1] : 0;
   a.channels = (int32_t)r.channels;
   a.states = (int32_t)states_;
   a.groups = (int32_t)groups;
   a.softplus = softplus;
-  a.n = a.rows = (int32_t)r.rows;
-  a.length = 1;
+  a.rows = (int32_t)r.rows;
+  if (a.length != 1) {
+    const size_t need = fav_selective_scan_workspace_bytes(&a);
+    if (need) {
+      if (workspace == g_none) return (int64_t)need;
+      Tensor w;
+      if (!w.read(workspace) || w.t.device_id != xt.t.device_id || w.t.ndim != 1 || !w.is(kDlUInt, 8) || !w.contiguous())
+        return kAsk;
+      a.workspace = (void*)w.data();
+      a.workspace_bytes = (size_t)w.t.shape[0];
+    }
+  }
   return fav_selective_scan(&a, stream);
 }
 
-int32_t fav_norm_rows_tensors(void* x, void* weight, void* bias, void* alpha, void* reciprocal, void* y, int32_t groups,
-                              float eps, int32_t activation) {
+int32_t fav_group_norm_tensors(void* x, void* weight, void* bias, void* alpha, void* reciprocal, void* offsets,
+                               void* status, void* y, int32_t groups, float eps, int32_t activation) {
   if (!g_exchange) return kAsk;
   Tensor xt;
   Rows r;
   fav_norm_args a{};
   void* stream = nullptr;
-  if (!xt.read(x) || (a.type = xt.type()) < 0 || xt.t.ndim != 2 || !rows_of(xt.t, &r) || groups < 1 ||
-      r.channels % groups || (activation == FAV_ACTIVATION_SNAKE) != (alpha != g_none) ||
-      (alpha != g_none) != (reciprocal != g_none) || !coefficients(weight, xt, {r.channels}, &a.weight) ||
+  if (!xt.read(x) || (a.type = xt.type()) < 0 || !rows_of(xt.t, &r) || groups < 1 || r.channels % groups ||
+      (activation == FAV_ACTIVATION_SNAKE) != (alpha != g_none) || (alpha != g_none) != (reciprocal != g_none) ||
+      !coefficients(weight, xt, {r.channels}, &a.weight) ||
       !coefficients(bias, xt, {r.channels}, &a.bias) || !coefficients(alpha, xt, {r.channels}, &a.alpha) ||
-      !coefficients(reciprocal, xt, {r.channels}, &a.reciprocal) || !same_rows(y, xt, &a.y, &a.y_stride) ||
-      !stream_of(xt, &stream))
+      !coefficients(reciprocal, xt, {r.channels}, &a.reciprocal) ||
+      !sequences_of(offsets, xt, r, &a.offsets, &a.n, &a.length) || !indices(status, xt, 1, &a.status) ||
+      !same_rows(y, xt, &a.y, &a.y_stride) || !stream_of(xt, &stream))
     return kAsk;
   a.x = xt.data();
   a.x_stride = r.stride;
@@ -258,8 +290,7 @@ int32_t fav_norm_rows_tensors(void* x, void* weight, void* bias, void* alpha, vo
   a.channels = (int32_t)r.channels;
   a.groups = groups;
   a.activation = activation;
-  a.n = a.rows = (int32_t)r.rows;
-  a.length = 1;
+  a.rows = (int32_t)r.rows;
   return fav_group_norm(&a, stream);
 }
 

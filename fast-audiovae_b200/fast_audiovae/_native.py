@@ -93,8 +93,8 @@ SIGNATURES = {
     "fav_project_int4": ([_P, _P], ct.c_int32),
     "fav_bind_tensors": ([_P, _P], ct.c_int32),
     "fav_causal_conv_tensors": ([ct.py_object] * 8 + [ct.c_int32], ct.c_int32),
-    "fav_scan_step_tensors": ([ct.py_object] * 12 + [ct.c_int32], ct.c_int32),
-    "fav_norm_rows_tensors": ([ct.py_object] * 6 + [ct.c_int32, ct.c_float, ct.c_int32], ct.c_int32),
+    "fav_selective_scan_tensors": ([ct.py_object] * 14 + [ct.c_int32], ct.c_int64),
+    "fav_group_norm_tensors": ([ct.py_object] * 8 + [ct.c_int32, ct.c_float, ct.c_int32], ct.c_int32),
     "fav_project_int4_tensors": ([ct.py_object] * 5 + [ct.c_int32], ct.c_int32),
     "fav_test_gemm": ([_P, ct.c_int32, ct.c_int32, _P, ct.c_int32, ct.c_int32, _P, _P], ct.c_int32),
     "fav_test_sine": ([_P, ct.c_int32, _P, _P], ct.c_int32),
@@ -142,7 +142,7 @@ def tensor_functions(tensor_type):
     if lib.fav_bind_tensors(pointer(capsule, b"dlpack_exchange_api"), id(None)) != 0:
         return None
     held = ct.PyDLL(str(LIBRARY))
-    for name in ("fav_causal_conv_tensors", "fav_scan_step_tensors", "fav_norm_rows_tensors",
+    for name in ("fav_causal_conv_tensors", "fav_selective_scan_tensors", "fav_group_norm_tensors",
                  "fav_project_int4_tensors"):
         fn = getattr(held, name)
         fn.argtypes, fn.restype = SIGNATURES[name]

@@ -275,12 +275,17 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
     is ``[N, channels]`` and finite, and ``d`` and ``dt_bias`` are ``[channels]``. N is 1 to
     128. ``state`` is ``[slots, 2, N, channels]`` fp32 (``scan_state``).
     """
-    if offsets is None:
-        native = _native_path(x, dt, a, b, c, d, z, dt_bias, state, codes, status, out)
-        if native is not None:
-            y = _empty_like(x) if out is None else out
-            if native.fav_scan_step_tensors(x, dt, a, b, c, d, z, dt_bias, state, codes, status, y, bool(softplus)) == 0:
-                return y
+    native = _native_path(x, dt, a, b, c, d, z, dt_bias, offsets, state, codes, status, out)
+    if native is not None:
+        y = _empty_like(x) if out is None else out
+        arrays = (x, dt, a, b, c, d, z, dt_bias, offsets, state, codes, status)
+        softplus = bool(softplus)
+        result = native.fav_selective_scan_tensors(*arrays, None, y, softplus)
+        if result > 64:
+            workspace = x.new_empty(result, dtype=torch.uint8)
+            result = native.fav_selective_scan_tensors(*arrays, workspace, y, softplus)
+        if result == 0:
+            return y
     kind, index = _main(x)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
@@ -338,12 +343,12 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     ``activation`` is None, ``"silu"`` or ``"snake"``, the decoder's
     ``v + reciprocal * sin(alpha * v)**2`` with ``[channels]`` coefficients.
     """
-    if offsets is None and status is None and type(groups) is int and activation in _ACTIVATIONS and eps >= 0:
-        native = _native_path(x, weight, bias, alpha, reciprocal, out)
+    if type(groups) is int and activation in _ACTIVATIONS and eps >= 0:
+        native = _native_path(x, weight, bias, alpha, reciprocal, offsets, status, out)
         if native is not None:
             y = _empty_like(x) if out is None else out
-            if native.fav_norm_rows_tensors(x, weight, bias, alpha, reciprocal, y, groups, eps,
-                                            _ACTIVATIONS[activation]) == 0:
+            if native.fav_group_norm_tensors(x, weight, bias, alpha, reciprocal, offsets, status, y, groups, eps,
+                                             _ACTIVATIONS[activation]) == 0:
                 return y
     kind, index = _main(x)
     shape, dtype = x.shape, x.dtype

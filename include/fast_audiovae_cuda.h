@@ -373,15 +373,17 @@ FAV_API int32_t fav_project_int4(const fav_int4_args *args, void *cuda_stream);
  * the tensors, check them as the functions above need them and launch on the
  * current stream of x's device. They return an fav_status, or -1 when a tensor
  * is not what the operator takes, or not on the current device: the binding then
- * checks for itself and says so. fav_scan_step_tensors and fav_norm_rows_tensors
- * take single rows ([rows][channels]) alone, which need no workspace. */
+ * checks for itself and says so. Where a scan needs a workspace and got None,
+ * fav_selective_scan_tensors returns its bytes (over 64) and has done nothing: the
+ * binding calls again with a uint8 tensor of that size. */
 FAV_API int32_t fav_bind_tensors(const void *exchange, void *none);
 FAV_API int32_t fav_causal_conv_tensors(void *x, void *weight, void *bias, void *offsets, void *state, void *codes,
                                         void *status, void *y, int32_t activation);
-FAV_API int32_t fav_scan_step_tensors(void *x, void *dt, void *a, void *b, void *c, void *d, void *z, void *dt_bias,
-                                      void *state, void *codes, void *status, void *y, int32_t softplus);
-FAV_API int32_t fav_norm_rows_tensors(void *x, void *weight, void *bias, void *alpha, void *reciprocal, void *y,
-                                      int32_t groups, float eps, int32_t activation);
+FAV_API int64_t fav_selective_scan_tensors(void *x, void *dt, void *a, void *b, void *c, void *d, void *z,
+                                           void *dt_bias, void *offsets, void *state, void *codes, void *status,
+                                           void *workspace, void *y, int32_t softplus);
+FAV_API int32_t fav_group_norm_tensors(void *x, void *weight, void *bias, void *alpha, void *reciprocal, void *offsets,
+                                       void *status, void *y, int32_t groups, float eps, int32_t activation);
 FAV_API int32_t fav_project_int4_tensors(void *x, void *weight, void *scales, void *bias, void *y, int32_t group);
 
 #ifdef __cplusplus

@@ -573,7 +573,10 @@ def test_both_ways_of_reading_tensors_agree(monkeypatch):
     x, q = normal(g, 6, 64, dtype=BF16).cuda(), torch.randint(0, 256, (48, 32), generator=g, dtype=torch.uint8).cuda()
     w, b = normal(g, 64, 4).cuda(), normal(g, 64).cuda()
     maps, a = normal(g, 6, 2, 8, dtype=BF16).cuda(), -torch.rand(8, 64, generator=g).cuda()
-    codes = codes_for(g, 6, 6).cuda()
+    codes, offsets = codes_for(g, 6, 6).cuda(), torch.tensor([0, 1, 1, 6], dtype=torch.int32, device="cuda")
+    # Long enough to be cut into pieces, with a map whose rows lie further apart.
+    long = [normal(g, 1, 2000, 64).cuda(), normal(g, 1, 2000, 64).cuda(), a,
+            normal(g, 1, 2000, 3, 8).cuda()[:, :, :2], normal(g, 1, 2000, 2, 8).cuda()]
     def run(kind):
         history, state = torch.ones(6, 2, 3, 64, dtype=BF16, device="cuda"), torch.ones(6, 2, 8, 64, device="cuda")
         first = x.as_subclass(Other) if kind == "subclass" else x
@@ -581,6 +584,11 @@ def test_both_ways_of_reading_tensors_agree(monkeypatch):
                 ops.causal_conv(first.view(2, 3, 64), w),
                 ops.selective_scan(first, x, a, maps, maps, d=b, z=x, dt_bias=b, state=state, codes=codes), state,
                 ops.group_norm(first, 8, b, b, activation="snake", alpha=b, reciprocal=b),
+                ops.group_norm(first.view(3, 2, 64), 8, b), ops.group_norm(first, 8, offsets=offsets),
+                ops.causal_conv(first, w, offsets=offsets),
+                ops.selective_scan(first.view(2, 3, 64), x.view(2, 3, 64), a, maps.view(2, 3, 2, 8), maps.view(2, 3, 2, 8)),
+                ops.selective_scan(first, x, a, maps, maps, offsets=offsets),
+                ops.selective_scan(*(t.as_subclass(Other) if kind == "subclass" and t is long[0] else t for t in long)),
                 ops.project_int4(first, q, torch.ones(48, 2, device="cuda"), w[:48, 0].contiguous(), group=32)]
     native = run("plain")
     assert ops._held, "tensors are not read natively here"
