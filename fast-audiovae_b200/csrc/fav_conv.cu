@@ -7,14 +7,16 @@
 // most recent inputs, in x's type) or are zero. Sums run in fp32, oldest tap
 // first, and round once to the output's type.
 //
-// A thread owns up to 16 bytes of neighbouring channels and walks down
+// A thread owns up to 4 neighbouring channels and walks down
 // `rows_per_thread` rows with the last K - 1 inputs in registers, so a tile
-// re-reads only the K - 1 rows above it. The next 16 rows are on their way to
+// re-reads only the K - 1 rows above it. The next 8 rows are on their way to
 // the thread's own ring in shared memory (cp.async): in registers they would
-// halve the resident warps. 33 ragged prompts of up to 750 x 2048 bf16 take 27 us,
-// 54 % of the copy rate: the SiLU's two special functions a value alone need 12
-// us, its other instructions 10, and the 16 warps an SM that the registers leave
-// overlap them in part. 512 single rows take 4.9 us.
+// halve the resident warps. Packs of 8 channels and rings of 16 rows leave 16
+// warps an SM instead of 32 and took 4 to 24 % longer on 16-bit prompts. 33 ragged
+// prompts of up to 750 x 2048 bf16 take 26 us, 57 % of the copy rate: the SiLU's
+// two special functions a value alone need 12 us, its other instructions 10, and
+// the resident warps overlap them in part. 64 x 2000 x 2048 without SiLU take 166
+// us, 97 %. 512 single rows take 4.9 us.
 #include "fav_common.cuh"
 #include "fav_ops.cuh"
 
@@ -22,7 +24,14 @@ namespace fav {
 namespace {
 
 constexpr int kConvThreads = 128;
-constexpr int kConvDepth = 16;  // rows of x on their way to a thread
+constexpr int kConvDepth = 8;  // rows of x on their way to a thread
+
+// Blocks that an SM holds at once. 64 registers a thread carry up to 4 taps;
+// more taps want 128 (16 x 750 x 2048 bf16, 8 taps: 41 us, with 80 and spills 52).
+template <int K>
+constexpr int conv_blocks() {
+  return K <= 4 ? 8 : 4;
+}
 
 struct ConvArgs {
   const void* x;
@@ -146,7 +155,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const __grid_co
 }
 
 template <typename T, int V, int K, bool ACT>
-__global__ void __launch_bounds__(kConvThreads, V == 8 ? 4 : 6) conv_kernel(const __grid_constant__ ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, conv_blocks<K>()) conv_kernel(const __grid_constant__ ConvArgs a) {
   constexpr int H = K - 1, U = 4, D = kConvDepth;
   using P = Pack<T, V>;
   // Each thread's next D rows: it copies, waits for and reads its own alone.
@@ -274,24 +283,16 @@ cudaError_t launch_taps(int taps, unsigned grid, cudaStream_t stream, const Conv
     case 2: return launch_act<T, V, 2>(grid, stream, a);
     case 3: return launch_act<T, V, 3>(grid, stream, a);
     case 4: return launch_act<T, V, 4>(grid, stream, a);
-    default: break;
+    case 5: return launch_act<T, V, 5>(grid, stream, a);
+    case 6: return launch_act<T, V, 6>(grid, stream, a);
+    case 7: return launch_act<T, V, 7>(grid, stream, a);
+    case 8: return launch_act<T, V, 8>(grid, stream, a);
+    default: return cudaErrorInvalidValue;
   }
-  if constexpr (V <= 4) {
-    switch (taps) {
-      case 5: return launch_act<T, V, 5>(grid, stream, a);
-      case 6: return launch_act<T, V, 6>(grid, stream, a);
-      case 7: return launch_act<T, V, 7>(grid, stream, a);
-      case 8: return launch_act<T, V, 8>(grid, stream, a);
-      default: break;
-    }
-  }
-  return cudaErrorInvalidValue;
 }
 
 template <typename T>
 cudaError_t launch_type(int taps, int v, unsigned grid, cudaStream_t stream, const ConvArgs& a) {
-  if constexpr (sizeof(T) == 2)
-    if (v == 8) return launch_taps<T, 8>(taps, grid, stream, a);
   return v == 4 ? launch_taps<T, 4>(taps, grid, stream, a) : launch_taps<T, 1>(taps, grid, stream, a);
 }
 
@@ -311,18 +312,17 @@ cudaError_t launch_causal_conv(const fav_conv_args& c, const Sequences& seq, cud
   a.silu = c.activation == FAV_ACTIVATION_SILU;
   const int elem = elem_bytes(c.type);
   a.step = !seq.offsets && seq.length == 1;
-  int v = c.type == FAV_TYPE_F32 || c.taps > 4 || a.step ? 4 : 8;
-  for (; v > 1; v = v == 8 ? 4 : 1)
-    if (c.channels % v == 0 && aligned_for(c.x, c.x_stride, elem, v) && aligned_for(c.y, c.y_stride, elem, v) &&
-        aligned_for(c.state_pool, 0, elem, v))
-      break;
+  const bool wide = c.channels % 4 == 0 && aligned_for(c.x, c.x_stride, elem, 4) &&
+                    aligned_for(c.y, c.y_stride, elem, 4) && aligned_for(c.state_pool, 0, elem, 4);
+  const int v = wide ? 4 : 1;
   const long long vecs = c.channels / v;
   a.wide_weight = aligned_for(c.weight, 0, 4, 4) && v * c.taps % 4 == 0;
-  // One wave of the 512 (V = 8) or 768 threads that an SM holds, so that every
-  // thread loads its coefficients and finds its sequence once; at most 64 rows a
-  // thread. Single rows: up to 4 a thread, for the coefficients.
-  const long long wave = 148LL * (v == 8 || a.step ? 512 : 768), most = a.step ? 4 : 64;
-  const long long rpt = ((long long)seq.rows * vecs + wave - 1) / wave;
+  // One wave of the threads that the SMs hold, so that every thread loads its
+  // coefficients and finds its sequence once; at most 64 rows a thread. Single
+  // rows: up to 4 a thread, for the coefficients.
+  const long long blocks_per_sm = c.taps <= 4 ? conv_blocks<4>() : conv_blocks<8>();
+  const long long wave = 148LL * kConvThreads * (a.step ? 4 : blocks_per_sm), most = a.step ? 4 : 64;
+  long long rpt = ((long long)seq.rows * vecs + wave - 1) / wave;
   a.rows_per_thread = (int)(rpt < 1 ? 1 : rpt > most ? most : rpt);
   a.row_tiles = (int)(((long long)seq.rows + a.rows_per_thread - 1) / a.rows_per_thread);
   const long long items = ((long long)a.row_tiles + (seq.offsets ? seq.n : 0)) * vecs;
