@@ -3,9 +3,13 @@
 // the sequence's rows and the group's channels, all of it in fp32.
 //
 // Variances are sums of squared differences from a mean, never a difference of
-// squares: a thread centres its values on its own mean, and threads and blocks
-// join by (count, mean, sum of squares about it), so a mean far from zero costs
-// no digits. The order of every sum is fixed.
+// squares. A running sum of values far from zero is off by its own roundings
+// (a clip of 6000 x 2048 values 1000.1 in one group: its mean by 0.004), so the pass
+// that sums the squares of x - mean sums those differences too: their mean corrects
+// both. A mean is kept as two floats, the second one part of the bias, and threads
+// and blocks join by (count, mean, sum of squares about it) with means as offsets
+// from one of them: a mean far from zero costs no digits but its square's in U.
+// The order of every sum is fixed.
 //
 // Bound by memory: x is read once and y written once. Single rows keep a group
 // in the registers of 1 to 256 threads. Longer sequences are cut into blocks of
@@ -97,10 +101,14 @@ struct NormChannels {
       pairs(re, a.recip, c, 0.f, a.wide);
     }
   }
-  // After load(): w times rstd, so that a value takes one multiply.
-  __device__ __forceinline__ void scale(float rstd) {
+  // After load(): w times rstd, so that a value takes one multiply, and the low part
+  // of the mean in the bias.
+  __device__ __forceinline__ void scale(float rstd, float low) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) w[i] = f2mul(w[i], make_float2(rstd, rstd));
+    for (int i = 0; i < P; ++i) {
+      w[i] = f2mul(w[i], make_float2(rstd, rstd));
+      b[i] = f2fma(w[i], make_float2(-low, -low), b[i]);
+    }
   }
   template <typename T>
   __device__ __forceinline__ Pack<T, V> apply(int activation, const Pack<T, V>& x, float mean) const {
@@ -145,35 +153,73 @@ __device__ __forceinline__ float2 add_values(const Pack<T, V>& x, float2 sum) {
   for (int i = 0; i < V / 2; ++i) sum = f2add(sum, pair_of(x, i));
   return sum;
 }
+// Sums of differences from a mean and of their squares, even and odd ones apart.
+struct Moments {
+  float2 sum, squares;
+};
 template <typename T, int V>
-__device__ __forceinline__ float2 add_squares(const Pack<T, V>& x, float mean, float2 sum) {
+__device__ __forceinline__ void add_moments(const Pack<T, V>& x, float mean, Moments& m) {
   if constexpr (V == 1) {
     const float d = to_f32(x.v[0]) - mean;
-    return make_float2(fmaf(d, d, sum.x), 0.f);
+    m.sum.x += d;
+    m.squares.x = fmaf(d, d, m.squares.x);
+    return;
   }
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) {
     const float2 d = f2add(pair_of(x, i), make_float2(-mean, -mean));
-    sum = f2fma(d, d, sum);
+    m.sum = f2add(m.sum, d);
+    m.squares = f2fma(d, d, m.squares);
   }
-  return sum;
 }
+// .x: the sum of the differences, .y: of their squares.
+__device__ __forceinline__ float2 total_of(const Moments& m) {
+  return make_float2(m.sum.x + m.sum.y, m.squares.x + m.squares.y);
+}
+
+// Of `count` values: their mean is mean + low, their squares are about that.
+struct Stats {
+  float mean, low, squares;
+};
+// From 1 / count and sums of differences from `about` (NaN stays NaN; rounding may
+// leave the squares of equal values just under zero).
+__device__ __forceinline__ Stats stats_of(float inv, float about, float2 sums) {
+  const float low = sums.x * inv;
+  return {about, low, max_nan(fmaf(-sums.x, low, sums.y), 0.f)};
+}
+// Joins the statistics `b` of `more` values to those of `count`; a's mean stays the
+// one that its low part counts from.
+__device__ __forceinline__ void join(Stats& a, float& count, const Stats& b, float more) {
+  if (more == 0.f) return;
+  const float n = count + more, d = (b.mean - a.mean) + b.low - a.low, f = more / n;
+  a.low = fmaf(d, f, a.low);
+  a.squares += b.squares + d * d * count * f;
+  count = n;
+}
+
+__device__ __forceinline__ float shuffle_add(float v, int o) { return v + __shfl_xor_sync(0xffffffffu, v, o); }
+__device__ __forceinline__ float2 shuffle_add(float2 v, int o) {
+  return make_float2(shuffle_add(v.x, o), shuffle_add(v.y, o));
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return f2add(a, b); }
 
 constexpr int kRowThreads = 256;  // single rows
 
 // ------------------------------------------------------------- single rows
 // `group_threads` threads (a power of two) hold a (row, group)'s values, NV
 // vectors each; NV = 0 reads them again instead.
-__device__ __forceinline__ float group_sum(float v, int threads, float* part) {
+template <typename S>
+__device__ __forceinline__ S group_sum(S v, int threads, S* part) {
   const int in_warp = min(threads, 32);
-  for (int o = in_warp / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = in_warp / 2; o > 0; o >>= 1) v = shuffle_add(v, o);
   if (threads > 32) {
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
     const int first = threadIdx.x / threads * (threads / 32);
-    v = 0.f;
-    for (int i = 0; i < threads / 32; ++i) v += part[first + i];
+    v = part[first];
+    for (int i = 1; i < threads / 32; ++i) v = add(v, part[first + i]);
   }
   return v;
 }
@@ -181,6 +227,7 @@ __device__ __forceinline__ float group_sum(float v, int threads, float* part) {
 template <typename T, int V, int NV>
 __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float part[kRowThreads / 32];
+  __shared__ float2 part2[kRowThreads / 32];
   grid_dependency_sync();
   const int threads = a.group_threads, per_block = kRowThreads / threads;
   const long long item = (long long)blockIdx.x * per_block + threadIdx.x / threads;
@@ -191,9 +238,10 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const __grid_con
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride + c0;
   T* y = static_cast<T*>(a.y) + row * a.y_stride + c0;
   const float inv = 1.f / (float)a.width;
+  Moments m{};
+  float2 sum = make_float2(0.f, 0.f);
   if constexpr (NV > 0) {
     Pack<T, V> xv[NV];
-    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (t + k * threads < vecs) {
@@ -201,31 +249,30 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const __grid_con
         sum = add_values(xv[k], sum);
       }
     const float mean = group_sum(sum.x + sum.y, threads, part) * inv;
-    sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (t + k * threads < vecs) sum = add_squares(xv[k], mean, sum);
-    const float rstd = rsqrtf(group_sum(sum.x + sum.y, threads, part) * inv + a.eps);
+      if (t + k * threads < vecs) add_moments(xv[k], mean, m);
+    const Stats s = stats_of(inv, mean, group_sum(total_of(m), threads, part2));
+    const float rstd = rsqrtf(s.squares * inv + a.eps);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (t + k * threads) * V;
       if (!live || t + k * threads >= vecs) continue;
       NormChannels<V> ch;
       ch.load(a, c0 + c);
-      ch.scale(rstd);
+      ch.scale(rstd, s.low);
       store_pack<T, V>(y + c, ch.apply(a.activation, xv[k], mean));
     }
   } else {
-    float2 sum = make_float2(0.f, 0.f);
     for (int k = t; k < vecs; k += threads) sum = add_values(load_const<T, V>(x + (size_t)k * V), sum);
     const float mean = group_sum(sum.x + sum.y, threads, part) * inv;
-    sum = make_float2(0.f, 0.f);
-    for (int k = t; k < vecs; k += threads) sum = add_squares(load_const<T, V>(x + (size_t)k * V), mean, sum);
-    const float rstd = rsqrtf(group_sum(sum.x + sum.y, threads, part) * inv + a.eps);
+    for (int k = t; k < vecs; k += threads) add_moments(load_const<T, V>(x + (size_t)k * V), mean, m);
+    const Stats s = stats_of(inv, mean, group_sum(total_of(m), threads, part2));
+    const float rstd = rsqrtf(s.squares * inv + a.eps);
     for (int k = t; live && k < vecs; k += threads) {
       NormChannels<V> ch;
       ch.load(a, c0 + k * V);
-      ch.scale(rstd);
+      ch.scale(rstd, s.low);
       store_pack<T, V>(y + (size_t)k * V, ch.apply(a.activation, load_const<T, V>(x + (size_t)k * V), mean));
     }
   }
@@ -242,33 +289,24 @@ constexpr int kMaxCtas = 16;  // of a cluster (above 8 where the device can plac
 // by vecs vectors, walked by threads in the order of e = row * vecs + vector. A
 // block of several groups has at most NT vectors, and only whole
 // rows of threads walk it: a thread then keeps to one vector, hence one group.
-template <int NT>
-__device__ __forceinline__ float block_sum(float v, float* part) {
+template <int NT, typename S>
+__device__ __forceinline__ S block_sum(S v, S* part) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 16; o > 0; o >>= 1) v = shuffle_add(v, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
+  v = part[0];
 #pragma unroll
-  for (int i = 0; i < NT / 32; ++i) v += part[i];
+  for (int i = 1; i < NT / 32; ++i) v = add(v, part[i]);
   return v;
-}
-
-struct Stats {
-  float count, mean, squares;
-};
-
-__device__ __forceinline__ Stats join(Stats a, Stats b) {
-  const float n = a.count + b.count;
-  if (b.count == 0.f) return a;
-  const float d = b.mean - a.mean, f = b.count / n;
-  return {n, fmaf(d, f, a.mean), a.squares + b.squares + d * d * a.count * f};
 }
 
 template <typename T, int V, int NT>
 __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(const __grid_constant__ NormArgs a) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  __shared__ float s_sum[NT], s_square[NT];
+  // A thread's statistics (several groups a block), then the groups' own.
+  __shared__ float s_mean[NT], s_low[NT], s_square[NT];
+  __shared__ float2 s_sums[NT / 32];
   using P = Pack<T, V>;
   P* kept = reinterpret_cast<P*>(s_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -342,55 +380,62 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
       if (v >= vecs) ++r, v -= vecs;
     }
   }
-  // Squares of this thread's values about `mean`.
-  const auto squares_about = [&](float mean) {
-    float2 s = make_float2(0.f, 0.f);
+  // This thread's differences from `mean` and their squares.
+  const auto moments_about = [&](float mean) {
+    Moments m{};
 #pragma unroll 4
-    for (int k = 0; k < kept_vectors; ++k) s = add_squares(kept[threadIdx.x + k * step], mean, s);
+    for (int k = 0; k < kept_vectors; ++k) add_moments(kept[threadIdx.x + k * step], mean, m);
     if (kept_vectors < vectors) {
       int r = r0, v = v0;
       for (int k = 0; k < vectors; ++k) {
-        if (k >= kept_vectors) s = add_squares(load_const<T, V>(x + r * a.x_stride + v * V), mean, s);
+        if (k >= kept_vectors) add_moments(load_const<T, V>(x + r * a.x_stride + v * V), mean, m);
         r += dr, v += dv;
         if (v >= vecs) ++r, v -= vecs;
       }
     }
-    return s.x + s.y;
+    return total_of(m);
   };
-  const float sum = sums.x + sums.y, all = (float)rows * (float)a.width;
+  const float sum = sums.x + sums.y, inv = rows ? 1.f / ((float)rows * (float)a.width) : 0.f;
   if (groups == 1) {
-    const float mean = rows ? block_sum<NT>(sum, s_sum) / all : 0.f;
-    const float squares = block_sum<NT>(squares_about(mean), s_square);
-    if (threadIdx.x == 0) s_stats[0] = {all, mean, squares};
+    const float mean = block_sum<NT>(sum, s_square) * inv;
+    const float2 total = block_sum<NT>(moments_about(mean), s_sums);
+    if (threadIdx.x == 0) s_stats[0] = stats_of(inv, mean, total);
   } else {
-    // A thread's squares are about its own mean. A warp joins a group's threads:
-    // the sum gives the mean, then the squares move to it.
-    const float n = (float)(vectors * V);
-    s_sum[threadIdx.x] = sum;
-    s_square[threadIdx.x] = vectors ? squares_about(sum / n) : 0.f;
+    // A thread's squares are about its own mean. A warp joins a group's threads, as
+    // seen from the mean of the group's first: the offsets give the group's mean,
+    // then the squares move to it.
+    Stats own{};
+    if (vectors) {
+      const float own_inv = 1.f / (float)(vectors * V), mean = sum * own_inv;
+      own = stats_of(own_inv, mean, moments_about(mean));
+    }
+    s_mean[threadIdx.x] = own.mean;
+    s_low[threadIdx.x] = own.low;
+    s_square[threadIdx.x] = own.squares;
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int g = warp; g < groups; g += NT / 32) {
-      float total = 0.f, squares = 0.f;
-      for (int i = lane; i < dr * group_vecs; i += 32) {
-        const int k = i / group_vecs;
-        total += s_sum[k * vecs + g * group_vecs + i - k * group_vecs];
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const float mean = rows ? total / all : 0.f;
-      for (int i = lane; i < dr * group_vecs; i += 32) {
-        const int k = i / group_vecs, t = k * vecs + g * group_vecs + i - k * group_vecs;
-        // Vectors that thread t walked: rows k, k + dr, ...
-        const int walked = rows > k ? (rows - k - 1) / dr + 1 : 0;
-        if (walked) {
-          const float nt = (float)(walked * V), d = s_sum[t] / nt - mean;
-          squares += fmaf(nt * d, d, s_square[t]);
+      const float origin = s_mean[g * group_vecs];
+      const auto each = [&](auto&& f) {  // f(values, mean's offset, squares) of the lane's threads
+        for (int i = lane; i < dr * group_vecs; i += 32) {
+          const int k = i / group_vecs, t = k * vecs + g * group_vecs + i - k * group_vecs;
+          // Vectors that thread t walked: rows k, k + dr, ...
+          const int walked = rows > k ? (rows - k - 1) / dr + 1 : 0;
+          if (walked) f((float)(walked * V), (s_mean[t] - origin) + s_low[t], s_square[t]);
         }
-      }
+      };
+      float total = 0.f, squares = 0.f;
+      each([&](float n, float offset, float) { total = fmaf(n, offset, total); });
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-      if (lane == 0) s_stats[g] = {all, mean, squares};
+      for (int o = 16; o > 0; o >>= 1) total = shuffle_add(total, o);
+      const float low = total * inv;
+      each([&](float n, float offset, float square) {
+        const float d = offset - low;
+        squares += fmaf(n * d, d, square);
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) squares = shuffle_add(squares, o);
+      if (lane == 0) s_stats[g] = {origin, low, squares};
     }
   }
   if (ctas > 1)
@@ -398,7 +443,6 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
   else
     __syncthreads();
   // Every CTA joins all of the cluster's, in order, into its own table.
-  float* s_mean = s_sum;
   float* s_rstd = s_square;
   if (threadIdx.x < groups) {  // at most one a thread
     const int g = threadIdx.x;
@@ -407,11 +451,13 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
     for (int i = 0; i < kMaxCtas; ++i)
       if (i < ctas) part[i] = cluster.map_shared_rank(s_stats, i)[g];
     Stats all = part[0];
+    float count = (float)min(share, length) * (float)a.width;
 #pragma unroll
     for (int i = 1; i < kMaxCtas; ++i)
-      if (i < ctas) all = join(all, part[i]);
+      if (i < ctas) join(all, count, part[i], (float)(min(share, length - min(i * share, length))) * (float)a.width);
     s_mean[g] = all.mean;
-    s_rstd[g] = all.count > 0.f ? rsqrtf(all.squares / all.count + a.eps) : 0.f;
+    s_low[g] = all.low;
+    s_rstd[g] = count > 0.f ? rsqrtf(all.squares / count + a.eps) : 0.f;
   }
   if (ctas > 1) cluster.barrier_arrive();  // done with the others' statistics
   __syncthreads();
@@ -421,7 +467,7 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
     const float mean = s_mean[g];
     NormChannels<V> ch;
     if (vectors) ch.load(a, c0 + v0 * V);
-    ch.scale(s_rstd[g]);
+    ch.scale(s_rstd[g], s_low[g]);
     T* p = y + r0 * a.y_stride + v0 * V;
     const long long hop = dr * a.y_stride;
 #pragma unroll 2
@@ -435,7 +481,7 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
       const P in = k < kept_vectors ? kept[threadIdx.x + k * step] : load_const<T, V>(x + r * a.x_stride + v * V);
       NormChannels<V> ch;
       ch.load(a, c0 + v * V);
-      ch.scale(s_rstd[0]);
+      ch.scale(s_rstd[0], s_low[0]);
       store_pack<T, V>(y + r * a.y_stride + v * V, ch.apply(a.activation, in, s_mean[0]));
       r += dr, v += dv;
       if (v >= vecs) ++r, v -= vecs;

@@ -1,0 +1,82 @@
+"""The stream operators at the ends of their range, on a B200 (``-m gpu``): far means, large sizes, extreme values."""
+import pytest
+import torch
+
+from fast_audiovae import _native, build, ops
+import ops_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    if not build.LIBRARY.exists():
+        build.build()
+    assert _native.load_library().fav_device_supported()
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def close(got, want, tol):
+    excess = (got.cpu().to(torch.float64) - want).abs() - tol
+    assert not torch.isnan(excess).any()
+    assert excess.max() <= 0, float(excess.max())
+
+
+# -------------------------------------------------------------- group_norm
+# Shape, groups, type, and the additions that a value passes through at most: the
+# vectors of a thread (two sums each), its warp, the block's warps and the cluster.
+# A cluster may have half the 16 CTAs that are asked for.
+FAR = [
+    ((1, 6000, 2048), 1, F32, 1600),   # 12.3e6 values, 8 or 16 x 512 threads, 4 a vector: 750 or 1500
+    ((1, 6000, 2048), 8, BF16, 400),   # 1.5e6 values, 16 or 8 CTAs of 128 threads at least, 8 a vector: 380
+    ((2, 750, 512), 1, F32, 100),
+    ((1, 3000, 32), 32, F32, 200),     # several groups a block: 8 threads a group
+    ((40, 100, 96), 8, F32, 200),
+    ((3, 333, 330), 11, F16, 200),
+    ((3, 40000), 1, F32, 200),         # single rows
+    ((5, 2048), 1, F32, 64),
+    ((7, 66), 22, F32, 64),
+]
+
+
+def norm_far_from_zero(x, groups, weight, bias, adds):
+    """The norm in float64 and a bound in which the mean enters by the square of a rounding alone.
+
+    A first sum errs by A = adds U of the values' size m, and so does the mean that the differences
+    are taken from: e = A m. Their own mean errs by A of the differences' size, spread + e, and so
+    does what is left of the mean. The squares err by A of their sum, which holds e^2.
+    """
+    u, wide = ref.U, x.to(ref.WIDE)
+    a = adds * u
+    part = wide.reshape(x.shape[0], -1, groups, x.shape[-1] // groups) if x.dim() == 3 else wide.reshape(
+        x.shape[0], 1, groups, -1)
+    mean = part.mean((1, 3), keepdim=True)
+    centred = part - mean
+    spread, size = (centred ** 2).mean((1, 3), keepdim=True), centred.abs().mean((1, 3), keepdim=True)
+    e = a * mean.abs()
+    left = (a + 2 * u) * (size + e)
+    spread_off = 3 * a * spread + 2 * left ** 2 + 4 * a * e ** 2
+    rstd = 1 / torch.sqrt(spread + 1e-5)
+    norm = centred * rstd
+    far = rstd * (left + 2 * u * (centred.abs() + e)) + norm.abs() * (spread_off * rstd ** 2 / 2 + 4 * u)
+    norm, far, e = ((t + 0 * part).reshape(x.shape) for t in (norm, far, e * rstd))
+    w, b = weight.to(ref.WIDE), bias.to(ref.WIDE)
+    y = norm * w + b
+    return y, far * w.abs() + 4 * u * ((norm * w).abs() + b.abs() + e * w.abs()) + ref.half_step(y, x.dtype)
+
+
+@pytest.mark.parametrize("shape,groups,dtype,adds", FAR)
+@pytest.mark.parametrize("value,spread", [(1000.1, 0.0), (10.1, 0.0), (1000.1, 0.01), (-300.7, 1.0)])
+def test_a_mean_far_from_zero_costs_group_norm_no_digits(shape, groups, dtype, adds, value, spread):
+    g = gen(sum(shape))
+    x = (value + spread * torch.randn(*shape, generator=g)).to(dtype)
+    weight, bias = torch.randn(shape[-1], generator=g), torch.randn(shape[-1], generator=g)
+    want, tol = norm_far_from_zero(x, groups, weight, bias, adds)
+    close(ops.group_norm(x.cuda(), groups, weight.cuda(), bias.cuda()), want, tol)
