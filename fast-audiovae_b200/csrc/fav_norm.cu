@@ -546,7 +546,7 @@ cudaError_t launch_sequences(NormArgs a, cudaStream_t stream) {
   a.block_groups = std::max(1, std::min(a.groups, 64 / (int)(a.width * sizeof(T))));
   while (a.block_groups > 1 && a.block_groups * vecs > 128) --a.block_groups;
   a.blocks = (a.groups + a.block_groups - 1) / a.block_groups;
-  const size_t row = (size_t)a.block_groups * a.width * sizeof(T), stats = a.block_groups * sizeof(Stats) + 16;
+  const size_t row = (size_t)a.block_groups * a.width * sizeof(T), stats = a.block_groups * sizeof(Stats);
   // Shared memory for sequences of up to twice the mean length.
   const long long rows = a.seq.offsets ? std::min<long long>(a.seq.rows, 2LL * a.seq.rows / a.seq.n + 1) : a.seq.length;
   // CTAs share a sequence while there are fewer than two an SM, or while a share
@@ -557,7 +557,8 @@ cudaError_t launch_sequences(NormArgs a, cudaStream_t stream) {
     ctas *= 2;
   const auto fit = [&] {
     const long long share = (rows + ctas - 1) / ctas;
-    a.keep_rows = (int)std::min<long long>(share, (kMaxNormSmem - stats) / row);
+    // (15: what rounding the rows up to 16 bytes may add)
+    a.keep_rows = (int)std::min<long long>(share, (kMaxNormSmem - stats - 15) / row);
     a.stats_at = (int)((a.keep_rows * row + 15) / 16 * 16);
     return a.stats_at + stats;
   };

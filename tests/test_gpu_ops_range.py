@@ -80,3 +80,11 @@ def test_a_mean_far_from_zero_costs_group_norm_no_digits(shape, groups, dtype, a
     weight, bias = torch.randn(shape[-1], generator=g), torch.randn(shape[-1], generator=g)
     want, tol = norm_far_from_zero(x, groups, weight, bias, adds)
     close(ops.group_norm(x.cuda(), groups, weight.cuda(), bias.cuda()), want, tol)
+
+
+# Rows that fill a CTA's shared memory to within 15 bytes of what it may ask for.
+@pytest.mark.parametrize("shape,groups", [((1, 54576, 48), 16), ((1, 81904, 20), 2), ((1, 6, 20477), 1)])
+def test_group_norm_of_rows_that_fill_the_shared_memory(shape, groups):
+    x = torch.randn(*shape, generator=gen(shape[1])).to(BF16)
+    want, tol = ref.group_norm(x[0], groups, None, None, 1e-5, None, None, None, [(0, shape[1])])
+    close(ops.group_norm(x.cuda(), groups)[0], want, tol)
