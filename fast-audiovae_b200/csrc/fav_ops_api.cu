@@ -166,8 +166,8 @@ int32_t fav_group_norm(const fav_norm_args* args, void* cuda_stream) {
   if (c.activation == FAV_ACTIVATION_SNAKE && (!c.alpha || !c.reciprocal))
     return fail(FAV_INVALID_ARGUMENT, "Snake needs alpha and reciprocal");
   if (!(c.eps >= 0.f)) return fail(FAV_INVALID_ARGUMENT, "eps must not be negative");
-  if (c.rows == 0 || c.n == 0) return FAV_OK;
-  if (!c.x || !c.y) return fail(FAV_INVALID_ARGUMENT, "NULL x or y");
+  if (c.n == 0) return FAV_OK;
+  if (c.rows && (!c.x || !c.y)) return fail(FAV_INVALID_ARGUMENT, "NULL x or y");
   if ((st = check_stride("x", c.x_stride, c.channels, c.rows)) != FAV_OK) return st;
   if ((st = check_stride("y", c.y_stride, c.channels, c.rows)) != FAV_OK) return st;
   const int e = elem_bytes(c.type);

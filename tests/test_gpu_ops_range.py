@@ -88,3 +88,11 @@ def test_group_norm_of_rows_that_fill_the_shared_memory(shape, groups):
     x = torch.randn(*shape, generator=gen(shape[1])).to(BF16)
     want, tol = ref.group_norm(x[0], groups, None, None, 1e-5, None, None, None, [(0, shape[1])])
     close(ops.group_norm(x.cuda(), groups)[0], want, tol)
+
+
+@pytest.mark.parametrize("offsets,code", [([0, 0, 0], 0), ([0, 0, 5], 0x201), ([3, 0], 0x201)])
+def test_group_norm_checks_the_offsets_of_no_rows(offsets, code):
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.group_norm(torch.empty(0, 64, device="cuda"), 4, offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"),
+                   status=status)
+    assert status.item() == code
