@@ -164,7 +164,7 @@ __device__ __forceinline__ Piece piece_at(const ScanArgs& a, int p) {
     r.first = r.seq * per;
     const int base = r.seq * q.length, end = base + q.length;
     r.begin = base + (p - r.first) * R;
-    r.end = min(r.begin + R, end);
+    r.end = (int)min((long long)r.begin + R, (long long)end);  // the sum may pass 32 bits
     r.last = r.end == end;
     r.ok = true;
     return r;

@@ -96,3 +96,18 @@ def test_group_norm_checks_the_offsets_of_no_rows(offsets, code):
     ops.group_norm(torch.empty(0, 64, device="cuda"), 4, offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"),
                    status=status)
     assert status.item() == code
+
+
+# ---------------------------------------------------------- selective_scan
+def test_selective_scan_of_over_two_to_the_30_rows():
+    """The last sequences of 20 million of 64 rows are those of a short call."""
+    n, length, last = 20_000_000, 64, 3
+    g = gen(30)
+    x, dt, b, c = (torch.zeros(n, length, *shape, dtype=BF16, device="cuda") for shape in ((1,), (1,), (1, 1), (1, 1)))
+    for t in (x, dt, b, c):
+        t[-last:] = torch.randn(last, *t.shape[1:], generator=g).to(BF16).cuda()
+    a = torch.tensor([[-0.5]], device="cuda")
+    y = ops.selective_scan(x, dt, a, b, c, out=torch.full_like(x, 7.0))
+    assert torch.equal(y[-last:], ops.selective_scan(*(t[-last:].contiguous() for t in (x, dt)), a,
+                                                     *(t[-last:].contiguous() for t in (b, c))))
+    assert not y[:-last].any()
