@@ -137,6 +137,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // v / (1 + e^-v) by the hardware's 2^x and 1/x (2 and 1 units in the last
 // place). Below -100, where e^-v overflows, v stands at -100: the result is

@@ -51,6 +51,14 @@ __device__ __forceinline__ float delta_of(const ScanArgs& a, float dt, int c) {
   return a.softplus ? softplus_f32(v) : v;
 }
 
+// h * 2^p over the rows of a piece, as row after row would give it: by thirds, whose
+// powers stay in range where 2^p does not and the product does (a growing state that
+// is still zero would become inf * 0). Beyond 2^+-378 any h but 0 is inf or 0.
+__device__ __forceinline__ float times_power(float h, float p) {
+  const float e = ex2_approx(min_nan(max_nan(p * 0.333333333f, -126.f), 126.f));
+  return h * e * e * e;
+}
+
 // ------------------------------------------------------------- single rows
 // One row per stream. Reading and writing the states is the whole cost (8 * N
 // bytes a channel), so a thread moves V = 4 neighbouring channels of a state
@@ -327,7 +335,7 @@ __global__ void __launch_bounds__(kBlockChannels* L, L == 2 ? 3 : 1) scan_kernel
       from += table;
       sums += a.channels;
       const float sum = *sums;
-      each([&](int j, size_t at) { h[j] = fmaf(ex2_approx(sum * decay[j]), h[j], from[at]); });
+      each([&](int j, size_t at) { h[j] = times_power(h[j], sum * decay[j]) + from[at]; });
     }
   }
   const float bias = a.dt_bias ? __ldg(a.dt_bias + c) : 0.f, skip = !PARTIAL && a.d ? __ldg(a.d + c) : 0.f;

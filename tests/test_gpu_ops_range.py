@@ -111,3 +111,40 @@ def test_selective_scan_of_over_two_to_the_30_rows():
     assert torch.equal(y[-last:], ops.selective_scan(*(t[-last:].contiguous() for t in (x, dt)), a,
                                                      *(t[-last:].contiguous() for t in (b, c))))
     assert not y[:-last].any()
+
+
+@pytest.mark.parametrize("rate,softplus", [(4.0, True), (-4.0, False)])
+def test_selective_scan_of_states_that_grow_late(rate, softplus):
+    """A state of zero stays zero however much it would grow; what grows at the end of a long prompt is finite.
+
+    Few prompts are cut into pieces of 32 rows, over which a state would grow by e^90, out of fp32's range; the
+    ten last rows, the only ones with inputs, let it grow by e^30.
+    """
+    rows, channels, states = 200, 64, 16
+    g = gen(31)
+    x, dt = torch.zeros(1, rows, channels), torch.rand(1, rows, channels, generator=g) * 0.1
+    x[:, -10:] = torch.randn(10, channels, generator=g)
+    a = torch.full((states, channels), rate)
+    if not softplus:
+        dt = -0.7 - dt
+    b, c = torch.randn(1, rows, 1, states, generator=g), torch.randn(1, rows, 1, states, generator=g)
+    want, tol, _, _ = ref.selective_scan(x[0], dt[0], a, b[0], c[0], None, None, None, softplus, [(0, rows)],
+                                         [torch.zeros(states, channels, dtype=ref.WIDE)])
+    close(ops.selective_scan(*(t.cuda() for t in (x, dt, a, b, c)), softplus=softplus)[0], want, tol)
+
+
+def test_selective_scan_of_states_that_fade():
+    """A large state without new inputs fades over a piece of a prompt as it does row by row, and no further."""
+    rows, channels, states = 200, 64, 16
+    x, maps, dt = torch.zeros(1, rows, channels), torch.ones(1, rows, 1, states), torch.zeros(1, rows, channels)
+    dt[:, 32:66] = 3.2     # 2^-148 over the second 32 rows
+    a = -torch.ones(states, channels)
+    pool = torch.full((1, 2, states, channels), 2.0 ** 120)
+    want, tol, new, new_tol = ref.selective_scan(x[0], dt[0], a, maps[0], maps[0], None, None, None, False, [(0, rows)],
+                                                 ref.states_before(pool, [0]))
+    dev = pool.cuda()
+    y = ops.selective_scan(*(t.cuda() for t in (x, dt, a, maps, maps)), softplus=False, state=dev,
+                           codes=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    close(y[0], want, tol)
+    assert (new[0] > 1e-12).all()
+    close(dev[0, 1], new[0], new_tol[0])
