@@ -24,8 +24,14 @@
 // their way at once, 16 bytes of weights a lane and row. (Twice and four times as
 // much, 1 x 64 x 4096 3.8 and 4.9 us instead of 3.4: straight code that runs once
 // costs more to fetch than the wait it saves.)
+// Sums of inputs times codes may leave fp32's range where the scaled ones do not
+// (bf16 and fp32 inputs above 2^117; fp16 stays far below). A thread that finds
+// such a sum forms it again, value by value and made smaller by 2^11: slow, but
+// out of the way of every other call.
 // Clusters that shared k and kept the inputs in shared memory took longer (7.0
 // us): the exchange costs more than the reads it saves.
+#include <type_traits>
+
 #include "fav_ops.cuh"
 
 namespace fav {
@@ -155,6 +161,24 @@ __device__ __forceinline__ Codes<W> load_codes(const uint8_t* p) {
   return c;
 }
 
+// A warp's share of one output, k blocks `block`, `block` + step, ... of `width` values, by
+// codes smaller and scales larger by 2^11, both exact: finite where the scaled sum is.
+template <typename T>
+__device__ __noinline__ float far_sum(const Int4Args& a, int row, int m, int block, int step, int width) {
+  const T* x = static_cast<const T*>(a.x) + m * a.x_stride;
+  const uint8_t* code = a.weight + (size_t)row * (a.depth / 2);
+  const float* scale = a.scales + (size_t)row * a.groups;
+  float sum = 0.f;
+  for (int k0 = block * width; k0 < a.depth; k0 += step * width) {
+    float part = 0.f;
+#pragma unroll 1
+    for (int k = k0; k < min(k0 + width, a.depth); ++k)
+      part = fmaf(to_f32(x[k]), (float)((code[k / 2] >> (k % 2 * 4) & 15) - 8) * 0x1p-11f, part);
+    sum = fmaf(scale[k0 / a.group] * 0x1p11f, part, sum);
+  }
+  return sum;
+}
+
 // R: tiles of 16 weight rows a warp; C: tiles of 8 input rows.
 template <typename T, bool WIDE, int W, int R, int C, int NW>
 __global__ void __launch_bounds__(32 * NW) int4_kernel(const __grid_constant__ Int4Args a) {
@@ -244,12 +268,26 @@ __global__ void __launch_bounds__(32 * NW) int4_kernel(const __grid_constant__ I
     }
   }
   // Accumulators 0, 1: weight row g, input rows 2 t and 2 t + 1; 2, 3: row g + 8.
+  bool over = false;
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s_sum[warp][8 * c + 2 * t + e % 2][16 * r + 8 * (e / 2) + g] = sum[r][c][e];
+      for (int e = 0; e < 4; ++e) {
+        s_sum[warp][8 * c + 2 * t + e % 2][16 * r + 8 * (e / 2) + g] = sum[r][c][e];
+        over |= !(fabsf(sum[r][c][e]) < INFINITY);
+      }
+  if constexpr (!std::is_same<T, __half>::value) {
+    if (over)
+#pragma unroll 1
+      for (int i = 0; i < R * C * 4; ++i) {
+        const int c = 8 * (i / 4 % C) + 2 * t + i % 2, r = 16 * (i / 4 / C) + 8 * (i / 2 % 2) + g;
+        float& v = s_sum[warp][c][r];
+        if (!(fabsf(v) < INFINITY) && m0 + c < a.rows && r0 + r < a.out)
+          v = far_sum<T>(a, r0 + r, m0 + c, warp, NW, KB);
+      }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < kIn * kOut; i += 32 * NW) {
     const int c = i / kOut, r = i % kOut, m = m0 + c, row = r0 + r;

@@ -148,3 +148,25 @@ def test_selective_scan_of_states_that_fade():
     close(y[0], want, tol)
     assert (new[0] > 1e-12).all()
     close(dev[0, 1], new[0], new_tol[0])
+
+
+# ------------------------------------------------------------ project_int4
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,out,depth,group", [(1, 333, 2048, 64), (9, 40, 608, 96), (20, 5000, 512, 128)])
+def test_project_int4_of_inputs_near_the_largest(rows, out, depth, group, dtype):
+    """Inputs of 10^38, whose sums times whole codes overflow, give their finite outputs; other rows keep their bits."""
+    g = gen(rows)
+    x = torch.randn(rows, depth, generator=g)
+    x[rows // 2] = (torch.rand(depth, generator=g) * 2 - 1) * 1e38
+    x = x.to(dtype)
+    weight = torch.randint(0, 256, (out, depth // 2), generator=g, dtype=torch.uint8)
+    scales = torch.rand(out, -(-depth // group), generator=g) * 0.001
+    bias = torch.randn(out, generator=g)
+    want, tol = ref.project_int4(x, weight, scales, bias, group)
+    assert want.abs().max() < 3e37
+    got = ops.project_int4(x.cuda(), weight.cuda(), scales.cuda(), bias.cuda(), group=group)
+    close(got, want, tol)
+    x[rows // 2] = 0
+    other = ops.project_int4(x.cuda(), weight.cuda(), scales.cuda(), bias.cuda(), group=group)
+    keep = [i for i in range(rows) if i != rows // 2]
+    assert torch.equal(got[keep], other[keep])
