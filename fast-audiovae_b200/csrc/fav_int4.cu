@@ -341,7 +341,7 @@ cudaError_t launch_type(const Int4Args& a, bool wide, cudaStream_t stream) {
 
 cudaError_t launch_project_int4(const fav_int4_args& c, cudaStream_t stream) {
   const Int4Args a{c.x, c.y, c.x_stride, c.y_stride, c.weight, c.scales, c.bias, c.rows, c.depth, c.out, c.group,
-             (c.depth + c.group - 1) / c.group};
+                   (int)(((long long)c.depth + c.group - 1) / c.group)};  // the sum may pass 32 bits
   const int elem = elem_bytes(c.type);
   const bool wide = aligned_for(c.x, c.x_stride, elem, 16 / elem);
   if (c.type == FAV_TYPE_F32) return launch_type<float>(a, wide, stream);

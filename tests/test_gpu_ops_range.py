@@ -170,3 +170,13 @@ def test_project_int4_of_inputs_near_the_largest(rows, out, depth, group, dtype)
     other = ops.project_int4(x.cuda(), weight.cuda(), scales.cuda(), bias.cuda(), group=group)
     keep = [i for i in range(rows) if i != rows // 2]
     assert torch.equal(got[keep], other[keep])
+
+
+@pytest.mark.parametrize("group", [2 ** 31 - 32, 2 ** 31 - 128, 2 ** 30])
+def test_project_int4_of_one_large_group(group):
+    """A group wider than the depth is one scale a row, however wide."""
+    g = gen(40)
+    x, weight = torch.randn(3, 96, generator=g).cuda(), torch.randint(0, 256, (70, 48), generator=g, dtype=torch.uint8)
+    scales = torch.rand(70, 1, generator=g)
+    want, tol = ref.project_int4(x.cpu(), weight, scales, None, 96)
+    close(ops.project_int4(x, weight.cuda(), scales.cuda(), group=group), want, tol)
