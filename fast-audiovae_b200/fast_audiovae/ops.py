@@ -51,6 +51,8 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "silu": 1, "snake": 2}
 _I32, _F32 = torch.int32, torch.float32
 _FRESH = 2
+_INT = 2 ** 31 - 1   # the library counts in 32 bits, to which ctypes would cut larger numbers
+_SLOTS = 2 ** 29
 _lib = None
 _grad_enabled = torch.is_grad_enabled
 _empty_like = torch.empty_like
@@ -172,14 +174,18 @@ def _sequences(shape, offsets, index):
         count = offsets.shape[0] if isinstance(offsets, torch.Tensor) and offsets.dim() else 0
         if count < 1:
             raise ValueError("offsets must hold n + 1 elements")
-        return count - 1, 0, shape[0], _index(offsets, "offsets", index, count)
-    if len(shape) == 2:
-        return shape[0], 1, shape[0], 0
-    if len(shape) == 3:
+        n, length, rows, at = count - 1, 0, shape[0], _index(offsets, "offsets", index, count)
+    elif len(shape) == 2:
+        n, length, rows, at = shape[0], 1, shape[0], 0
+    elif len(shape) == 3:
         if shape[1] < 1:
             raise ValueError("Sequences without offsets must have at least one row")
-        return shape[0], shape[1], shape[0] * shape[1], 0
-    raise ValueError("x must have shape [rows, channels] or [n, length, channels]")
+        n, length, rows, at = shape[0], shape[1], shape[0] * shape[1], 0
+    else:
+        raise ValueError("x must have shape [rows, channels] or [n, length, channels]")
+    if n > _INT or rows > _INT or shape[-1] > _INT:
+        raise ValueError("x has too many rows or channels: each below 2^31")
+    return n, length, rows, at
 
 
 def _states(state, codes, dtype, index, n, shape):
@@ -197,6 +203,8 @@ def _states(state, codes, dtype, index, n, shape):
         raise ValueError(f"state must be a contiguous {dtype} tensor of shape {['slots', *shape]} on x's device")
     if held[0] < n:
         raise ValueError(f"{n} sequences need at least as many slots; state has {held[0]}")
+    if held[0] > _SLOTS:
+        raise ValueError("state has too many slots: up to 2^29")
     return state.data_ptr(), _index(codes, "codes", index, n), held[0]
 
 
@@ -343,7 +351,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     ``activation`` is None, ``"silu"`` or ``"snake"``, the decoder's
     ``v + reciprocal * sin(alpha * v)**2`` with ``[channels]`` coefficients.
     """
-    if type(groups) is int and activation in _ACTIVATIONS and eps >= 0:
+    if type(groups) is int and groups <= _INT and activation in _ACTIVATIONS and eps >= 0:
         native = _native_path(x, weight, bias, alpha, reciprocal, offsets, status, out)
         if native is not None:
             y = _empty_like(x) if out is None else out
@@ -394,7 +402,8 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
     depth are multiples of 32.
     """
     native = _native_path(x, weight, scales, bias, out)
-    if native is not None and type(group) is int and weight is not None and x.dim() == 2 and weight.dim() == 2:
+    if (native is not None and type(group) is int and group <= _INT and weight is not None and x.dim() == 2
+            and weight.dim() == 2):
         y = x.new_empty((x.shape[0], weight.shape[0])) if out is None else out
         if native.fav_project_int4_tensors(x, weight, scales, bias, y, group) == 0:
             return y
@@ -419,7 +428,11 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
     if scales is None:
         raise ValueError("scales are required")
     width = packed[0]
+    if rows > _INT or depth > _INT or width > _INT:
+        raise ValueError("x or weight is too large: each size below 2^31")
     scales_at = _vector(scales, "scales", index, (width, -(-depth // group)))
+    if group > _INT:   # one scale a row, as for any group that is wider than the depth
+        group = 2 ** 30
     bias_at = _vector(bias, "bias", index, (width,))
     x_at, x_stride = _array(x, "x", dtype, index, shape)
     if _grad_enabled() and (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)):

@@ -180,3 +180,15 @@ def test_project_int4_of_one_large_group(group):
     scales = torch.rand(70, 1, generator=g)
     want, tol = ref.project_int4(x.cpu(), weight, scales, None, 96)
     close(ops.project_int4(x, weight.cuda(), scales.cuda(), group=group), want, tol)
+
+
+def test_numbers_beyond_32_bits_are_not_cut():
+    x = torch.randn(3, 64, device="cuda")
+    weight, scales = torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.ones(8, 2, device="cuda")
+    with pytest.raises(ValueError, match="divides the channels"):
+        ops.group_norm(x, 2 ** 32 + 4)
+    with pytest.raises(ValueError, match="scales must be"):
+        ops.project_int4(x, weight, scales, group=2 ** 32 + 32)
+    for group in (2 ** 31, 2 ** 32 + 32):
+        assert torch.equal(ops.project_int4(x, weight, scales[:, 0].unsqueeze(1).contiguous(), group=group),
+                           ops.project_int4(x, weight, scales[:, 0].unsqueeze(1).contiguous(), group=128))
