@@ -40,6 +40,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _native
 from ._native import CONV_ARGS, INT4_ARGS, NORM_ARGS, SCAN_ARGS
@@ -72,7 +73,7 @@ _held = False  # not looked for yet; None where the tensors cannot be read nativ
 def _native_path(*tensors):
     """The native entry points, if all of ``tensors`` are plain ones without gradients, or None but for the first."""
     global _held
-    if tensors[0] is None:
+    if tensors[0] is None or _forward._current_level >= 0:
         return None
     if _held is False:
         _held = _native.tensor_functions(torch.Tensor) if torch.cuda.is_available() else None
@@ -116,8 +117,13 @@ def _main(x):
         raise ValueError("x must be a float32, bfloat16 or float16 tensor") from None
 
 
-def _no_gradients():
-    raise RuntimeError("Stream operators have no gradients; call them under torch.no_grad()")
+def _no_gradients(*tensors):
+    """Refuses tensors, inputs and outputs alike, that want gradients or carry forward derivatives."""
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor) and t.is_floating_point()]
+    if _grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("Stream operators have no gradients; call them under torch.no_grad()")
+    if _forward._current_level >= 0 and any(_forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("Stream operators have no gradients, forward ones neither; detach their tensors")
 
 
 def _array(t, name, dtype, index, shape):
@@ -224,6 +230,7 @@ def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=No
                                           _ACTIVATIONS[activation]) == 0:
             return y
     kind, index = _main(x)
+    _no_gradients(x, weight, bias, state, out)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
@@ -237,8 +244,6 @@ def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=No
     x_at, x_stride = _array(x, "x", dtype, index, shape)
     pool_at, codes_at, slots = _states(state, codes, dtype, index, n, (2, taps - 1, channels))
     status_at = _index(status, "status", index, 1) if status is not None else 0
-    if _grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        _no_gradients()
     lib = _library(index)
     if out is None:  # contiguous: x's rows have one stride, or lie that way themselves
         out = _empty_like(x)
@@ -295,6 +300,7 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
         if result == 0:
             return y
     kind, index = _main(x)
+    _no_gradients(x, dt, a, b, c, d, z, dt_bias, state, out)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
@@ -315,10 +321,6 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
     bias_at = _vector(dt_bias, "dt_bias", index, (channels,))
     pool_at, codes_at, slots = _states(state, codes, _F32, index, n, (2, states, channels))
     status_at = _index(status, "status", index, 1) if status is not None else 0
-    if _grad_enabled() and (x.requires_grad or dt.requires_grad or a.requires_grad or b.requires_grad or c.requires_grad or
-                            (d is not None and d.requires_grad) or (z is not None and z.requires_grad) or
-                            (dt_bias is not None and dt_bias.requires_grad)):
-        _no_gradients()
     lib = _library(index)
     if out is None:  # contiguous: x's rows have one stride, or lie that way themselves
         out = _empty_like(x)
@@ -359,6 +361,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
                                              _ACTIVATIONS[activation]) == 0:
                 return y
     kind, index = _main(x)
+    _no_gradients(x, weight, bias, alpha, reciprocal, out)
     shape, dtype = x.shape, x.dtype
     n, length, rows, offsets_at = _sequences(shape, offsets, index)
     channels = shape[-1]
@@ -375,10 +378,6 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
                     _vector(alpha, "alpha", index, per), _vector(reciprocal, "reciprocal", index, per))
     x_at, x_stride = _array(x, "x", dtype, index, shape)
     status_at = _index(status, "status", index, 1) if status is not None else 0
-    if _grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                            (bias is not None and bias.requires_grad) or
-                            (alpha is not None and (alpha.requires_grad or reciprocal.requires_grad))):
-        _no_gradients()
     lib = _library(index)
     if out is None:  # contiguous: x's rows have one stride, or lie that way themselves
         out = _empty_like(x)
@@ -408,6 +407,7 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
         if native.fav_project_int4_tensors(x, weight, scales, bias, y, group) == 0:
             return y
     kind, index = _main(x)
+    _no_gradients(x, scales, bias, out)
     shape, dtype = x.shape, x.dtype
     if len(shape) != 2:
         raise ValueError("x must have shape [rows, depth]")
@@ -435,8 +435,6 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
         group = 2 ** 30
     bias_at = _vector(bias, "bias", index, (width,))
     x_at, x_stride = _array(x, "x", dtype, index, shape)
-    if _grad_enabled() and (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)):
-        _no_gradients()
     lib = _library(index)
     if out is None:
         out = x.new_empty((rows, width))

@@ -192,3 +192,19 @@ def test_numbers_beyond_32_bits_are_not_cut():
     for group in (2 ** 31, 2 ** 32 + 32):
         assert torch.equal(ops.project_int4(x, weight, scales[:, 0].unsqueeze(1).contiguous(), group=group),
                            ops.project_int4(x, weight, scales[:, 0].unsqueeze(1).contiguous(), group=128))
+
+
+def test_forward_derivatives_of_device_tensors_are_refused():
+    x, w, state = torch.ones(2, 64, device="cuda"), torch.ones(64, 4, device="cuda"), ops.conv_state(2, 64, 4, dtype=F32)
+    want = ops.causal_conv(x, w)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no gradients"):
+            ops.causal_conv(torch.autograd.forward_ad.make_dual(x, x), w)
+        assert torch.equal(ops.causal_conv(x, w), want)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.func.jvp(lambda t: ops.causal_conv(t, w), (x,), (x,))
+    codes = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.causal_conv(x, w, state=state.requires_grad_(), codes=codes)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.causal_conv(x, w, out=torch.empty_like(x).requires_grad_())

@@ -27,3 +27,45 @@ def wide(*shape, dtype=torch.float32):
 def test_sizes_beyond_32_bits_are_refused(call, words):
     with pytest.raises(ValueError, match=words):
         call()
+
+
+X, W, Q, S = torch.zeros(6, 64), torch.zeros(64, 4), torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2)
+MAPS, A, CODES = torch.zeros(6, 1, 4), torch.zeros(4, 64), torch.zeros(6, dtype=torch.int32)
+CALLS = [   # a call by its floating point tensors
+    (lambda x, w, b, h, out: ops.causal_conv(x, w, b, state=h, codes=CODES, out=out),
+     [X, W, torch.zeros(64), torch.zeros(6, 2, 3, 64), X]),
+    (lambda x, dt, a, b, c, d, z, bias, h, out: ops.selective_scan(x, dt, a, b, c, d=d, z=z, dt_bias=bias, state=h,
+                                                                  codes=CODES, out=out),
+     [X, X, A, MAPS, MAPS, torch.zeros(64), X, torch.zeros(64), torch.zeros(6, 2, 4, 64), X]),
+    (lambda x, w, b, alpha, r, out: ops.group_norm(x, 4, w, b, activation="snake", alpha=alpha, reciprocal=r, out=out),
+     [X] + [torch.zeros(64)] * 4 + [X]),
+    (lambda x, s, b, out: ops.project_int4(x, Q, s, b, group=32, out=out), [X, S, torch.zeros(8), torch.zeros(6, 8)]),
+]
+PLACES = [(call, tensors, i) for call, tensors in CALLS for i in range(len(tensors))]
+
+
+@pytest.mark.parametrize("call,tensors,place", PLACES)
+def test_gradients_of_any_tensor_are_refused(call, tensors, place):
+    """Reverse and forward ones, of inputs, states and outputs."""
+    def given(t):
+        return [t if i == place else other for i, other in enumerate(tensors)]
+    leaf = tensors[place].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        call(*given(leaf))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+        call(*given(leaf))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(tensors[place].clone(), torch.ones_like(tensors[place]))
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call(*given(dual))
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call(*tensors)
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="no CPU path"):
+            call(*(t.clone() for t in tensors))
+
+
+def test_derivatives_of_functions_are_refused():
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.func.jvp(lambda x: ops.causal_conv(x, W), (X,), (X,))
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.func.grad(lambda x: ops.causal_conv(x, W).sum())(X)
