@@ -67,6 +67,8 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 # points that read and check them natively (a fifth of the time that it takes from
 # here). What those do not take is checked below, which also says what is wrong.
 _KINDS = {torch.Tensor, torch.nn.Parameter, type(None)}
+# What the exchange raises of a tensor without plain memory (sparse, quantised, nested).
+_UNREADABLE = (RuntimeError, BufferError)
 _held = False  # not looked for yet; None where the tensors cannot be read natively
 
 
@@ -109,12 +111,23 @@ def _call(lib, function, args, index):
 
 # The checks below run on every call of a step that takes microseconds, so they
 # read each tensor attribute once. One that is missing is a ValueError too.
+_MISSING = (AttributeError, KeyError, TypeError, RuntimeError)
+
+
 def _main(x):
     """Checks an operator's first argument; returns its type code and device index."""
     try:
-        return _TYPES[x.dtype], x.get_device()
-    except (AttributeError, KeyError, TypeError):
-        raise ValueError("x must be a float32, bfloat16 or float16 tensor") from None
+        kind, index = _TYPES[x.dtype], x.get_device()
+        if _dense(x, x.dtype, index):
+            return kind, index
+    except _MISSING:
+        pass
+    raise ValueError("x must be a dense float32, bfloat16 or float16 tensor")
+
+
+def _dense(t, dtype, index):
+    """Whether t lies in plain memory of device ``index``."""
+    return t.dtype is dtype and t.get_device() == index and t.layout is torch.strided and not t.is_nested
 
 
 def _no_gradients(*tensors):
@@ -129,8 +142,8 @@ def _no_gradients(*tensors):
 def _array(t, name, dtype, index, shape):
     """Address and row stride of an array of x's type with adjacent channels."""
     try:
-        good = t.dtype is dtype and t.get_device() == index and t.shape == shape
-    except AttributeError:
+        good = _dense(t, dtype, index) and t.shape == shape
+    except _MISSING:
         good = False
     if not good:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)} on x's device")
@@ -156,18 +169,18 @@ def _vector(t, name, index, shape):
     if t is None:
         return 0
     try:
-        if t.dtype is _F32 and t.get_device() == index and t.shape == shape and t.is_contiguous():
+        if _dense(t, _F32, index) and t.shape == shape and t.is_contiguous():
             return t.data_ptr()
-    except AttributeError:
+    except _MISSING:
         pass
     raise ValueError(f"{name} must be a contiguous float32 tensor of shape {list(shape)} on x's device")
 
 
 def _index(t, name, index, count):
     try:
-        if t.dtype is _I32 and t.get_device() == index and t.shape == (count,) and t.is_contiguous():
+        if _dense(t, _I32, index) and t.shape == (count,) and t.is_contiguous():
             return t.data_ptr()
-    except AttributeError:
+    except _MISSING:
         pass
     raise ValueError(f"{name} must be a contiguous int32 tensor of {count} elements on x's device")
 
@@ -202,8 +215,8 @@ def _states(state, codes, dtype, index, n, shape):
         raise ValueError("state and codes go together")
     try:
         held = state.shape
-        good = state.dtype is dtype and state.get_device() == index and held[1:] == shape and state.is_contiguous()
-    except AttributeError:
+        good = _dense(state, dtype, index) and held[1:] == shape and state.is_contiguous()
+    except _MISSING:
         good = False
     if not good:
         raise ValueError(f"state must be a contiguous {dtype} tensor of shape {['slots', *shape]} on x's device")
@@ -225,10 +238,13 @@ def causal_conv(x, weight, bias=None, *, activation=None, offsets=None, state=No
     """
     native = _native_path(x, weight, bias, offsets, state, codes, status, out)
     if native is not None and (activation is None or activation == "silu"):
-        y = _empty_like(x) if out is None else out
-        if native.fav_causal_conv_tensors(x, weight, bias, offsets, state, codes, status, y,
-                                          _ACTIVATIONS[activation]) == 0:
-            return y
+        try:
+            y = _empty_like(x) if out is None else out
+            if native.fav_causal_conv_tensors(x, weight, bias, offsets, state, codes, status, y,
+                                              _ACTIVATIONS[activation]) == 0:
+                return y
+        except _UNREADABLE:
+            pass
     kind, index = _main(x)
     _no_gradients(x, weight, bias, state, out)
     shape, dtype = x.shape, x.dtype
@@ -261,8 +277,8 @@ def _maps(t, name, dtype, index, lead, groups, states):
     """Address, row stride and group stride of an input or output map."""
     shape = (*lead, groups, states)
     try:
-        good = t.dtype is dtype and t.get_device() == index and t.shape == shape
-    except AttributeError:
+        good = _dense(t, dtype, index) and t.shape == shape
+    except _MISSING:
         good = False
     if not good:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)} on x's device")
@@ -290,15 +306,18 @@ def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, softplus=Tru
     """
     native = _native_path(x, dt, a, b, c, d, z, dt_bias, offsets, state, codes, status, out)
     if native is not None:
-        y = _empty_like(x) if out is None else out
         arrays = (x, dt, a, b, c, d, z, dt_bias, offsets, state, codes, status)
         softplus = bool(softplus)
-        result = native.fav_selective_scan_tensors(*arrays, None, y, softplus)
-        if result > 64:
-            workspace = x.new_empty(result, dtype=torch.uint8)
-            result = native.fav_selective_scan_tensors(*arrays, workspace, y, softplus)
-        if result == 0:
-            return y
+        try:
+            y = _empty_like(x) if out is None else out
+            result = native.fav_selective_scan_tensors(*arrays, None, y, softplus)
+            if result > 64:
+                workspace = x.new_empty(result, dtype=torch.uint8)
+                result = native.fav_selective_scan_tensors(*arrays, workspace, y, softplus)
+            if result == 0:
+                return y
+        except _UNREADABLE:
+            pass
     kind, index = _main(x)
     _no_gradients(x, dt, a, b, c, d, z, dt_bias, state, out)
     shape, dtype = x.shape, x.dtype
@@ -356,10 +375,13 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     if type(groups) is int and groups <= _INT and activation in _ACTIVATIONS and eps >= 0:
         native = _native_path(x, weight, bias, alpha, reciprocal, offsets, status, out)
         if native is not None:
-            y = _empty_like(x) if out is None else out
-            if native.fav_group_norm_tensors(x, weight, bias, alpha, reciprocal, offsets, status, y, groups, eps,
-                                             _ACTIVATIONS[activation]) == 0:
-                return y
+            try:
+                y = _empty_like(x) if out is None else out
+                if native.fav_group_norm_tensors(x, weight, bias, alpha, reciprocal, offsets, status, y, groups, eps,
+                                                 _ACTIVATIONS[activation]) == 0:
+                    return y
+            except _UNREADABLE:
+                pass
     kind, index = _main(x)
     _no_gradients(x, weight, bias, alpha, reciprocal, out)
     shape, dtype = x.shape, x.dtype
@@ -403,9 +425,12 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
     native = _native_path(x, weight, scales, bias, out)
     if (native is not None and type(group) is int and group <= _INT and weight is not None and x.dim() == 2
             and weight.dim() == 2):
-        y = x.new_empty((x.shape[0], weight.shape[0])) if out is None else out
-        if native.fav_project_int4_tensors(x, weight, scales, bias, y, group) == 0:
-            return y
+        try:
+            y = x.new_empty((x.shape[0], weight.shape[0])) if out is None else out
+            if native.fav_project_int4_tensors(x, weight, scales, bias, y, group) == 0:
+                return y
+        except _UNREADABLE:
+            pass
     kind, index = _main(x)
     _no_gradients(x, scales, bias, out)
     shape, dtype = x.shape, x.dtype
@@ -416,9 +441,9 @@ def project_int4(x, weight, scales, bias=None, *, group, out=None):
         raise ValueError("group and the depth must be positive multiples of 32")
     try:
         packed = weight.shape
-        good = (weight.dtype is torch.uint8 and weight.get_device() == index and len(packed) == 2
-                and packed[1] == depth // 2 and weight.is_contiguous())
-    except AttributeError:
+        good = (_dense(weight, torch.uint8, index) and len(packed) == 2 and packed[1] == depth // 2
+                and weight.is_contiguous())
+    except _MISSING:
         good = False
     if not good:
         raise ValueError(f"weight must be a contiguous uint8 tensor of shape ['out', {depth // 2}] on x's device")

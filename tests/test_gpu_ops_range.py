@@ -208,3 +208,13 @@ def test_forward_derivatives_of_device_tensors_are_refused():
         ops.causal_conv(x, w, state=state.requires_grad_(), codes=codes)
     with pytest.raises(RuntimeError, match="no gradients"):
         ops.causal_conv(x, w, out=torch.empty_like(x).requires_grad_())
+
+
+def test_device_tensors_without_plain_memory_are_refused():
+    x, w = torch.ones(6, 64, device="cuda"), torch.ones(64, 4, device="cuda")
+    for call in (lambda: ops.causal_conv(x.to_sparse(), w), lambda: ops.causal_conv(x, w.to_sparse()),
+                 lambda: ops.causal_conv(x, w, out=x.to_sparse()), lambda: ops.group_norm(x.to_sparse(), 4),
+                 lambda: ops.group_norm(x, 4, w[:, 0].to_sparse()),
+                 lambda: ops.project_int4(x.to_sparse(), torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), w[:8, :2], group=32)):
+        with pytest.raises(ValueError, match="must be"):
+            call()

@@ -2,9 +2,15 @@
 import pytest
 import torch
 
-from fast_audiovae import ops
+from fast_audiovae import _native, build, ops
 
 MANY = 2 ** 31
+
+
+@pytest.fixture(scope="module", autouse=True)
+def library():
+    if not build.LIBRARY.exists():
+        build.build()
 
 
 def wide(*shape, dtype=torch.float32):
@@ -69,3 +75,36 @@ def test_derivatives_of_functions_are_refused():
         torch.func.jvp(lambda x: ops.causal_conv(x, W), (X,), (X,))
     with pytest.raises(RuntimeError, match="no gradients"):
         torch.func.grad(lambda x: ops.causal_conv(x, W).sum())(X)
+
+
+@pytest.fixture
+def native_reading(monkeypatch):
+    """Tensors go through the native entry points first, which leave those of the CPU to the caller."""
+    held = _native.tensor_functions(torch.Tensor)
+    assert held
+    monkeypatch.setattr(ops, "_held", held)
+
+
+def without_plain_memory(t):
+    yield t.to_sparse()
+    yield t.to_mkldnn()
+    yield torch.quantize_per_tensor(t, 0.1, 0, torch.qint8)
+    yield torch.nested.nested_tensor([t, t], layout=torch.strided)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("native", [False, True])
+def test_tensors_without_plain_memory_are_refused(native, request):
+    """Whichever tensor it is, and whichever way it is read, with the reason."""
+    if native:
+        request.getfixturevalue("native_reading")
+    for call, tensors in CALLS:
+        for i, t in enumerate(tensors[:-1]):   # outputs are looked at on the device
+            for odd in without_plain_memory(t):
+                with pytest.raises(ValueError, match="must be|must have"):
+                    call(*(odd if j == i else other for j, other in enumerate(tensors)))
+    for name in ("offsets", "status"):
+        with pytest.raises(ValueError, match=f"{name} must"):
+            ops.causal_conv(X, W, **{name: CODES.to_sparse()})
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.causal_conv(X, W)
