@@ -41,7 +41,18 @@ void* g_none = nullptr;
 struct Tensor {
   DlTensor t;
   bool read(void* object) {  // false of None too, which the exchange must not be given
-    return object != g_none && g_exchange->view(object, &t) == 0 && t.device_type == kDlCuda && t.strides && t.lanes == 1;
+    return object != g_none && g_exchange->view(object, &t) == 0 && t.device_type == kDlCuda && t.strides &&
+           t.lanes == 1 && !may_be_negated();
+  }
+  // The exchange does not tell whether a tensor stands for the negative of its memory. Such
+  // a one is the imaginary part of conjugated numbers, every second value of a row: with
+  // adjacent channels it has one channel, and lies apart or is a single value. The caller
+  // looks closer.
+  bool may_be_negated() const {
+    if (t.ndim == 0 || t.shape[t.ndim - 1] != 1 || (t.code != kDlFloat && t.code != kDlBfloat)) return false;
+    int64_t count = 1;
+    for (int i = 0; i < t.ndim; ++i) count *= t.shape[i];
+    return count == 1 || !contiguous();
   }
   const char* data() const { return static_cast<const char*>(t.data) + t.byte_offset; }
   bool is(uint8_t code, uint8_t bits) const { return t.code == code && t.bits == bits; }

@@ -126,8 +126,9 @@ def _main(x):
 
 
 def _dense(t, dtype, index):
-    """Whether t lies in plain memory of device ``index``."""
-    return t.dtype is dtype and t.get_device() == index and t.layout is torch.strided and not t.is_nested
+    """Whether t lies in plain memory of device ``index`` (which a negated view does not stand for)."""
+    return (t.dtype is dtype and t.get_device() == index and t.layout is torch.strided and not t.is_nested
+            and not t.is_neg())
 
 
 def _no_gradients(*tensors):

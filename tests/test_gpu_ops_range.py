@@ -218,3 +218,15 @@ def test_device_tensors_without_plain_memory_are_refused():
                  lambda: ops.project_int4(x.to_sparse(), torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), w[:8, :2], group=32)):
         with pytest.raises(ValueError, match="must be"):
             call()
+
+
+def test_negated_views_of_device_tensors_are_refused():
+    """The imaginary part of conjugated numbers: its memory holds the opposite sign. Other strided rows of one run."""
+    z = torch.complex(torch.arange(6.0), torch.arange(6.0)).cuda()
+    w = torch.tensor([[0.0, 1.0]], device="cuda")
+    assert torch.equal(ops.causal_conv(z.imag[:, None], w), z.imag[:, None])
+    for call in (lambda: ops.causal_conv(z.conj().imag[:, None], w),
+                 lambda: ops.causal_conv(z.imag[:, None], w, z[:1].conj().imag),
+                 lambda: ops.causal_conv(z.imag[:, None], w, out=z.conj().imag[:, None])):
+        with pytest.raises(ValueError, match="must be"):
+            call()

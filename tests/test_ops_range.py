@@ -108,3 +108,26 @@ def test_tensors_without_plain_memory_are_refused(native, request):
             ops.causal_conv(X, W, **{name: CODES.to_sparse()})
     with pytest.raises(RuntimeError, match="no CPU path"):
         ops.causal_conv(X, W)
+
+
+def negated(t):
+    """t as the negative of its memory: the imaginary part of conjugated numbers."""
+    return torch.complex(torch.zeros_like(t), -t).conj().imag
+
+
+@pytest.mark.parametrize("native", [False, True])
+def test_negated_views_are_refused(native, request):
+    """Their memory holds the opposite sign."""
+    if native:
+        request.getfixturevalue("native_reading")
+    rows, one = torch.arange(6.0), torch.ones(1)
+    x = rows[:, None]
+    assert torch.equal(negated(rows), rows) and negated(rows).is_neg()
+    maps = x.unsqueeze(2)
+    for call in (lambda: ops.causal_conv(negated(rows)[:, None], torch.ones(1, 4)),
+                 lambda: ops.causal_conv(x, torch.ones(1, 4), negated(one)),
+                 lambda: ops.selective_scan(x, x, one[None], negated(rows)[:, None, None], maps),
+                 lambda: ops.group_norm(x, 1, negated(one)),
+                 lambda: ops.project_int4(torch.zeros(1, 64), Q[:1], negated(one)[None], group=64)):
+        with pytest.raises(ValueError, match="must be"):
+            call()
