@@ -1,6 +1,8 @@
 // C ABI of the stream operators: argument checks, then the launches of
 // fav_conv.cu, fav_scan.cu, fav_norm.cu and fav_int4.cu. Declarations and
 // contracts: include/fast_audiovae_cuda.h.
+#include <initializer_list>
+
 #include "fav_ops.cuh"
 
 namespace fav {
@@ -62,6 +64,14 @@ int32_t check_stride(const char* name, int64_t stride, int32_t width, int32_t ro
   return FAV_OK;
 }
 
+// A load from an address that is no multiple of its size would fault on the device.
+int32_t check_aligned(int bytes, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % bytes)
+      return fail(FAV_INVALID_ARGUMENT, "array at %p is not aligned to its elements of %d bytes", p, bytes);
+  return FAV_OK;
+}
+
 int32_t launched(cudaError_t e, const char* what) {
   if (e == cudaErrorInvalidValue) return fail(FAV_SIZE_OVERFLOW, "%s too large", what);
   return e == cudaSuccess ? FAV_OK : cuda_fail(e, what);
@@ -102,6 +112,9 @@ int32_t fav_causal_conv(const fav_conv_args* args, void* cuda_stream) {
   if ((st = check_stride("x", c.x_stride, c.channels, c.rows)) != FAV_OK) return st;
   if ((st = check_stride("y", c.y_stride, c.channels, c.rows)) != FAV_OK) return st;
   const int e = elem_bytes(c.type);
+  if ((st = check_aligned(e, {c.x, c.y, c.state_pool})) != FAV_OK ||
+      (st = check_aligned(4, {c.weight, c.bias, c.slot_codes, c.offsets, c.status})) != FAV_OK)
+    return st;
   const long long state = 2LL * (c.taps - 1) * c.channels;
   const View x = view(c.x, c.x_stride, c.channels, c.rows, e), y = view(c.y, c.y_stride, c.channels, c.rows, e);
   const View pool = view(c.state_pool, state, state, c.num_slots, e);
@@ -141,6 +154,9 @@ int32_t fav_selective_scan(const fav_scan_args* args, void* cuda_stream) {
   if (need && (!c.workspace || c.workspace_bytes < need))
     return fail(FAV_INVALID_ARGUMENT, "workspace too small: %zu < %zu bytes", c.workspace ? c.workspace_bytes : 0, need);
   const int e = elem_bytes(c.type);
+  if ((st = check_aligned(e, {c.x, c.dt, c.z, c.b, c.c, c.y})) != FAV_OK ||
+      (st = check_aligned(4, {c.a, c.d, c.dt_bias, c.state_pool, c.slot_codes, c.offsets, c.status, c.workspace})) != FAV_OK)
+    return st;
   const long long state = 2LL * c.states * c.channels;
   const View y = view(c.y, c.y_stride, c.channels, c.rows, e);
   const View pool = view(c.state_pool, state, state, c.num_slots, 4);
@@ -171,6 +187,9 @@ int32_t fav_group_norm(const fav_norm_args* args, void* cuda_stream) {
   if ((st = check_stride("x", c.x_stride, c.channels, c.rows)) != FAV_OK) return st;
   if ((st = check_stride("y", c.y_stride, c.channels, c.rows)) != FAV_OK) return st;
   const int e = elem_bytes(c.type);
+  if ((st = check_aligned(e, {c.x, c.y})) != FAV_OK ||
+      (st = check_aligned(4, {c.weight, c.bias, c.alpha, c.reciprocal, c.offsets, c.status})) != FAV_OK)
+    return st;
   if (overlap(view(c.x, c.x_stride, c.channels, c.rows, e), view(c.y, c.y_stride, c.channels, c.rows, e)))
     return fail(FAV_OVERLAP, "x and y must not overlap");
   return launched(launch_group_norm(c, sequences(c.offsets, nullptr, c.n, c.length, c.rows, 0, c.status),
@@ -193,6 +212,7 @@ int32_t fav_project_int4(const fav_int4_args* args, void* cuda_stream) {
   if ((st = check_stride("y", c.y_stride, c.out, c.rows)) != FAV_OK) return st;
   if (reinterpret_cast<uintptr_t>(c.weight) % 16) return fail(FAV_INVALID_ARGUMENT, "weight must be 16-byte aligned");
   const int e = elem_bytes(c.type);
+  if ((st = check_aligned(e, {c.x, c.y})) != FAV_OK || (st = check_aligned(4, {c.scales, c.bias})) != FAV_OK) return st;
   if (overlap(view(c.x, c.x_stride, c.depth, c.rows, e), view(c.y, c.y_stride, c.out, c.rows, e)))
     return fail(FAV_OVERLAP, "x and y must not overlap");
   return launched(launch_project_int4(c, static_cast<cudaStream_t>(cuda_stream)), "projection");

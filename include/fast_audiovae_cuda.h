@@ -256,7 +256,8 @@ FAV_API int32_t fav_test_sine(const float *x, int32_t n, float *out, void *cuda_
  * pools with two tables a slot, slot codes, a device status word).
  *
  * Rows and sequences. Arrays are [rows][channels] with a row stride in
- * elements and adjacent channels. `offsets` (device int32[n + 1]) gives
+ * elements and adjacent channels, aligned to their elements (4-bit weights to 16
+ * bytes); others are refused. `offsets` (device int32[n + 1]) gives
  * sequence i the rows offsets[i] .. offsets[i + 1]; a sequence may have none,
  * and rows before the first or behind the last are left as they are. With
  * NULL offsets every sequence has `length` rows (rows = n * length); length 1

@@ -1,4 +1,6 @@
 """Stream operators without a GPU: sizes beyond 32 bits, kinds of tensors, gradients, alignment."""
+import ctypes as ct
+
 import pytest
 import torch
 
@@ -131,3 +133,34 @@ def test_negated_views_are_refused(native, request):
                  lambda: ops.project_int4(torch.zeros(1, 64), Q[:1], negated(one)[None], group=64)):
         with pytest.raises(ValueError, match="must be"):
             call()
+
+
+FAR = 1 << 24   # no two of the arrays below meet
+ARRAYS = {      # fields of the element type, and of 4 bytes
+    "fav_causal_conv": ("x y state_pool", "weight bias slot_codes offsets status"),
+    "fav_selective_scan": ("x dt z b c y", "a d dt_bias state_pool slot_codes offsets status workspace"),
+    "fav_group_norm": ("x y", "weight bias alpha reciprocal offsets status"),
+    "fav_project_int4": ("x y", "scales bias"),
+}
+SIZES = {
+    "fav_causal_conv": (_native.ConvArgs, dict(x_stride=8, y_stride=8, channels=8, taps=4, n=2, rows=6, num_slots=2)),
+    "fav_selective_scan": (_native.ScanArgs, dict(x_stride=8, dt_stride=8, z_stride=8, b_stride=4, c_stride=4, y_stride=8,
+                                                  channels=8, states=4, groups=1, n=2, rows=6, num_slots=2)),
+    "fav_group_norm": (_native.NormArgs, dict(x_stride=8, y_stride=8, channels=8, groups=2, n=2, rows=6, eps=1e-5)),
+    "fav_project_int4": (_native.Int4Args, dict(x_stride=64, y_stride=8, weight=1 << 20, rows=2, depth=64, out=8, group=32)),
+}
+
+
+@pytest.mark.parametrize("name", list(ARRAYS))
+@pytest.mark.parametrize("kind,size", [(0, 4), (1, 2), (2, 2)])
+def test_arrays_off_their_elements_are_refused(name, kind, size):
+    """Every array of the C ABI, at each address between two elements; such a load would fault."""
+    lib = _native.load_library()
+    struct, sizes = SIZES[name]
+    rows, words = (fields.split() for fields in ARRAYS[name])
+    arrays = {field: FAR * (i + 1) for i, field in enumerate(rows + words)}
+    for field, width in [(f, size) for f in rows] + [(f, 4) for f in words]:
+        for off in range(1, width):
+            args = struct(type=kind, **sizes, **{**arrays, field: arrays[field] + off})
+            assert getattr(lib, name)(ct.byref(args), None) == 1, (field, off)
+            assert b"aligned" in lib.fav_last_error()
