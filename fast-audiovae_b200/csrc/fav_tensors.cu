@@ -7,6 +7,8 @@
 #include "../../include/fast_audiovae_cuda.h"
 #include "fav_internal.h"
 
+#include <dlfcn.h>
+
 #include <initializer_list>
 
 namespace fav {
@@ -37,6 +39,20 @@ constexpr uint8_t kDlInt = 0, kDlUInt = 1, kDlFloat = 2, kDlBfloat = 4;
 
 const DlExchange* g_exchange = nullptr;
 void* g_none = nullptr;
+
+// The interpreter's lock, which a launch gives back meanwhile: it waits while the
+// device's queue is full, and the program's other threads need not. The functions
+// are the running interpreter's own.
+void* (*g_save)() = nullptr;
+void (*g_restore)(void*) = nullptr;
+int (*g_locked)() = nullptr;
+
+struct Unlocked {
+  void* thread = g_save && g_restore && g_locked && g_locked() ? g_save() : nullptr;
+  ~Unlocked() {
+    if (thread) g_restore(thread);
+  }
+};
 
 struct Tensor {
   DlTensor t;
@@ -210,6 +226,9 @@ int32_t fav_bind_tensors(const void* exchange, void* none) {
   if (e->major != 1 || !e->view || !e->current_stream) return fail(FAV_UNSUPPORTED, "DLPack 1.x exchange required");
   g_exchange = e;
   g_none = none;
+  g_save = reinterpret_cast<void* (*)()>(dlsym(RTLD_DEFAULT, "PyEval_SaveThread"));
+  g_restore = reinterpret_cast<void (*)(void*)>(dlsym(RTLD_DEFAULT, "PyEval_RestoreThread"));
+  g_locked = reinterpret_cast<int (*)()>(dlsym(RTLD_DEFAULT, "PyGILState_Check"));
   return FAV_OK;
 }
 
@@ -234,6 +253,7 @@ int32_t fav_causal_conv_tensors(void* x, void* weight, void* bias, void* offsets
   a.taps = (int32_t)taps;
   a.activation = activation;
   a.rows = (int32_t)r.rows;
+  Unlocked meanwhile;
   return fav_causal_conv(&a, stream);
 }
 
@@ -277,6 +297,7 @@ int64_t fav_selective_scan_tensors(void* x, void* dt, void* a_, void* b, void* c
       a.workspace_bytes = (size_t)w.t.shape[0];
     }
   }
+  Unlocked meanwhile;
   return fav_selective_scan(&a, stream);
 }
 
@@ -302,6 +323,7 @@ int32_t fav_group_norm_tensors(void* x, void* weight, void* bias, void* alpha, v
   a.groups = groups;
   a.activation = activation;
   a.rows = (int32_t)r.rows;
+  Unlocked meanwhile;
   return fav_group_norm(&a, stream);
 }
 
@@ -329,6 +351,7 @@ int32_t fav_project_int4_tensors(void* x, void* weight, void* scales, void* bias
   a.depth = (int32_t)r.channels;
   a.out = (int32_t)out;
   a.group = group;
+  Unlocked meanwhile;
   return fav_project_int4(&a, stream);
 }
 

@@ -132,8 +132,8 @@ def load_library(path=None):
 
 
 def tensor_functions(tensor_type):
-    """The entry points that read tensor objects themselves, as functions that keep the interpreter's
-    lock; None when ``tensor_type`` has no DLPack 1.x C exchange interface."""
+    """The entry points that read tensor objects themselves, as functions that are called with the
+    interpreter's lock (which they give back while they launch); None when ``tensor_type`` has no DLPack 1.x C exchange interface."""
     lib = load_library()
     capsule = getattr(tensor_type, "__dlpack_c_exchange_api__", None)
     if capsule is None:

@@ -372,7 +372,7 @@ FAV_API int32_t fav_project_int4(const fav_int4_args *args, void *cuda_stream);
  * framework whose DLPack C exchange interface (DLPack 1.x,
  * `dlpack_exchange_api`) was bound, or None (`none`) for an absent one. They read
  * the tensors, check them as the functions above need them and launch on the
- * current stream of x's device. They return an fav_status, or -1 when a tensor
+ * current stream of x's device, without the lock while they launch. They return an fav_status, or -1 when a tensor
  * is not what the operator takes, or not on the current device: the binding then
  * checks for itself and says so. Where a scan needs a workspace and got None,
  * fav_selective_scan_tensors returns its bytes (over 64) and has done nothing: the

@@ -1,4 +1,7 @@
 """The stream operators at the ends of their range, on a B200 (``-m gpu``): far means, large sizes, extreme values."""
+import threading
+import time
+
 import pytest
 import torch
 
@@ -230,3 +233,32 @@ def test_negated_views_of_device_tensors_are_refused():
                  lambda: ops.causal_conv(z.imag[:, None], w, out=z.conj().imag[:, None])):
         with pytest.raises(ValueError, match="must be"):
             call()
+
+
+def test_other_threads_run_while_a_call_waits_for_the_queue():
+    """Calls into a full queue wait for the device, but not with the interpreter's lock."""
+    x, w, out = torch.ones(2, 64, device="cuda"), torch.ones(64, 4, device="cuda"), torch.empty(2, 64, device="cuda")
+    ops.causal_conv(x, w, out=out)
+    torch.cuda.synchronize()
+    done, gaps = threading.Event(), []
+
+    def tick():
+        last = time.perf_counter()
+        while not done.is_set():
+            time.sleep(0.002)
+            now = time.perf_counter()
+            gaps.append(now - last)
+            last = now
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    torch.cuda._sleep(1_500_000_000)   # most of a second, and it ends by itself
+    begin = time.perf_counter()
+    for _ in range(8000):
+        ops.causal_conv(x, w, out=out)
+    took = time.perf_counter() - begin
+    done.set()
+    thread.join()
+    torch.cuda.synchronize()
+    assert took > 0.4, "the queue never filled"
+    assert max(gaps) < 0.2, max(gaps)
