@@ -514,7 +514,9 @@ class StreamSlots:
     step advance together: ``codes(slots)`` before the step, and
     ``commit(slots)`` once it has succeeded. A step that is not committed
     leaves every state as it was. Slots start afresh until their first commit
-    and again after ``reset``.
+    and again after ``reset``. Codes are uploaded without waiting for the device;
+    the upload is no part of a captured step, whose codes are written before its
+    replay (``out``).
     """
 
     def __init__(self, slots, *, device="cuda"):
@@ -536,11 +538,22 @@ class StreamSlots:
             raise ValueError("A slot may appear only once per step")
         return index
 
-    def codes(self, slots):
-        """The slot codes of a step over distinct ``slots``, on the device."""
+    def codes(self, slots, out=None):
+        """The slot codes of a step over distinct ``slots``, on the device, in ``out`` if given."""
         index = self._checked(slots)
-        codes = (index.astype(np.int32) << 2) | (self._fresh[index] * _FRESH) | self._table[index]
-        return torch.from_numpy(codes).to(self.device)
+        if out is not None and not (isinstance(out, torch.Tensor) and out.dtype is _I32 and out.shape == index.shape
+                                    and out.is_contiguous() and out.device.type == self.device.type):
+            raise ValueError(f"out must be a contiguous int32 tensor of {index.size} elements on the slots' device")
+        codes = torch.from_numpy(
+            (index.astype(np.int32) << 2) | (self._fresh[index] * _FRESH) | self._table[index])
+        if self.device.type == "cuda":
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("A capture would keep these codes for good; write the codes of a replay into "
+                                   "the captured tensor before it (out=)")
+            codes = codes.pin_memory()   # its allocator keeps the memory until the copy from it is done
+        if out is None:
+            return codes.to(self.device, non_blocking=True)
+        return out.copy_(codes, non_blocking=True)
 
     def commit(self, slots):
         index = self._checked(slots)

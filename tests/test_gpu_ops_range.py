@@ -262,3 +262,29 @@ def test_other_threads_run_while_a_call_waits_for_the_queue():
     torch.cuda.synchronize()
     assert took > 0.4, "the queue never filled"
     assert max(gaps) < 0.2, max(gaps)
+
+
+def test_codes_do_not_wait_for_the_device():
+    """Codes of many steps, made while the stream is busy, arrive as they were."""
+    slots, streams = ops.StreamSlots(512), list(range(512))
+    out = torch.empty(512, dtype=torch.int32, device="cuda")
+    slots.codes(streams)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_000_000_000)   # about half a second
+    begin, got, want = time.perf_counter(), [], []
+    for step in range(40):
+        got.append(slots.codes(streams) if step % 2 else slots.codes(streams, out=out).clone())
+        want.append([i << 2 | (0 if step else 2) | step % 2 for i in streams])
+        slots.commit(streams)
+    assert time.perf_counter() - begin < 0.2
+    assert torch.equal(torch.stack(got).cpu(), torch.tensor(want, dtype=torch.int32))
+
+
+def test_codes_are_no_part_of_a_capture():
+    slots, x, graph = ops.StreamSlots(4), torch.zeros(2, device="cuda"), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="before it"):
+            slots.codes([0, 1])
+    graph.replay()
+    assert x.tolist() == [1.0, 1.0]

@@ -164,3 +164,11 @@ def test_arrays_off_their_elements_are_refused(name, kind, size):
             args = struct(type=kind, **sizes, **{**arrays, field: arrays[field] + off})
             assert getattr(lib, name)(ct.byref(args), None) == 1, (field, off)
             assert b"aligned" in lib.fav_last_error()
+
+
+def test_codes_into_a_given_tensor():
+    slots, out = ops.StreamSlots(4, device="cpu"), torch.zeros(2, dtype=torch.int32)
+    assert slots.codes([3, 1], out=out) is out and out.tolist() == [3 << 2 | 2, 1 << 2 | 2]
+    for bad in (torch.zeros(3, dtype=torch.int32), torch.zeros(2), torch.zeros(4, dtype=torch.int32)[::2], [0, 0]):
+        with pytest.raises(ValueError, match="out must be"):
+            slots.codes([3, 1], out=bad)
