@@ -9,12 +9,14 @@
 
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace fav {
 namespace {
 
 constexpr int32_t kAsk = -1;
+constexpr size_t kMinWorkspace = 256;  // what a scan asks for at least: above every status
 
 // DLPack 1.x: the structures of its C interface that are used here.
 struct DlTensor {
@@ -289,7 +291,7 @@ int64_t fav_selective_scan_tensors(void* x, void* dt, void* a_, void* b, void* c
   if (a.length != 1) {
     const size_t need = fav_selective_scan_workspace_bytes(&a);
     if (need) {
-      if (workspace == g_none) return (int64_t)need;
+      if (workspace == g_none) return (int64_t)std::max(need, kMinWorkspace);
       Tensor w;
       if (!w.read(workspace) || w.t.device_id != xt.t.device_id || w.t.ndim != 1 || !w.is(kDlUInt, 8) || !w.contiguous())
         return kAsk;

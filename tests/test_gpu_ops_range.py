@@ -288,3 +288,11 @@ def test_codes_are_no_part_of_a_capture():
             slots.codes([0, 1])
     graph.replay()
     assert x.tolist() == [1.0, 1.0]
+
+
+def test_a_scan_asks_for_small_workspaces_natively_too():
+    """A prompt of one channel and two states needs 36 bytes."""
+    ops.group_norm(torch.ones(1, 64, device="cuda"), 4)
+    x, maps = torch.ones(1, 65, 1, device="cuda"), torch.ones(1, 65, 1, 2, device="cuda")
+    args = x, x, -torch.ones(2, 1, device="cuda"), maps, maps, *[None] * 7
+    assert ops._held.fav_selective_scan_tensors(*args, None, torch.empty_like(x), False) > 64
