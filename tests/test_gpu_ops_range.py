@@ -296,3 +296,42 @@ def test_a_scan_asks_for_small_workspaces_natively_too():
     x, maps = torch.ones(1, 65, 1, device="cuda"), torch.ones(1, 65, 1, 2, device="cuda")
     args = x, x, -torch.ones(2, 1, device="cuda"), maps, maps, *[None] * 7
     assert ops._held.fav_selective_scan_tensors(*args, None, torch.empty_like(x), False) > 64
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_calls_see_what_their_own_stream_wrote(native, monkeypatch):
+    """On a busy side stream an input is written late, with other data each time: a call that did not wait for
+    that stream would read what was there before (NaN at first), whichever way its tensors are read."""
+    g = gen(50)
+    if not native:
+        monkeypatch.setattr(ops, "_held", None)
+    w, a = torch.randn(64, 4, generator=g).cuda(), -torch.rand(4, 64, generator=g).cuda()
+    weight, scales = torch.randint(0, 256, (40, 32), generator=g, dtype=torch.uint8).cuda(), torch.ones(40, 2, device="cuda")
+    data = torch.randn(5, 400, 64, generator=g).cuda()
+    x = torch.empty(400, 64, device="cuda")
+    pool, codes = torch.zeros(400, 2, 3, 64, device="cuda"), (torch.arange(400, dtype=torch.int32) << 2).cuda()
+
+    def run():
+        maps = x[:, :4].unsqueeze(1)
+        return [ops.causal_conv(x, w, state=pool, codes=codes), pool, ops.causal_conv(x[None], w), ops.group_norm(x, 8),
+                ops.group_norm(x[None], 8), ops.selective_scan(x, x, a, maps, maps),
+                ops.selective_scan(x[None], x[None], a, maps[None], maps[None]),   # cut into pieces, two launches
+                ops.project_int4(x, weight, scales, group=32)]
+
+    want = []
+    for rows in data:
+        x.copy_(rows)
+        want.append([t.clone() for t in run()])
+    x.fill_(float("nan"))
+    torch.cuda.synchronize()
+    side, got = torch.cuda.Stream(), []
+    with torch.cuda.stream(side):
+        for rows in data:
+            torch.cuda._sleep(20_000_000)   # ten milliseconds
+            x.copy_(rows)
+            got.append([t.clone() for t in run()])
+            x.fill_(float("nan"))
+    side.synchronize()
+    for one, other in zip(want, got):
+        for t, u in zip(one, other):
+            assert torch.equal(t, u)
