@@ -66,7 +66,7 @@ __device__ __forceinline__ Pack<T, V> narrow(const Row<V>& r) {
 }
 
 // A thread's coefficients, and one row of y from the K rows that end at it.
-template <int V, int K, bool ACT>
+template <typename T, int V, int K, bool ACT>
 struct ConvThread {
   static constexpr int P = (V + 1) / 2;
   float2 w[K][P], bias[P];
@@ -98,7 +98,7 @@ struct ConvThread {
       float2 v = bias[p];
 #pragma unroll
       for (int j = 0; j < K; ++j) v = f2fma(w[j][p], win[j].v[p], v);
-      out.v[p] = ACT ? silu2(v) : v;
+      out.v[p] = ACT ? silu2<T>(v) : v;
     }
     return out;
   }
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const __grid_co
   T* y = static_cast<T*>(a.y) + c;
   T* pool = static_cast<T*>(a.pool) + c;
   const int first = (int)tile * a.rows_per_thread, last = min(first + a.rows_per_thread, q.rows);
-  ConvThread<V, K, ACT> th;
+  ConvThread<T, V, K, ACT> th;
   th.load(a, c);
   for (int r0 = first; r0 < last; r0 += U) {
     P win[U][K];
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kConvThreads, conv_blocks<K>()) conv_kernel(co
     copy_commit();
     px += a.x_stride;
   }
-  ConvThread<V, K, ACT> th;
+  ConvThread<T, V, K, ACT> th;
   th.load(a, c);
   Row<V> win[H + U];
   Span sp{0, 0};

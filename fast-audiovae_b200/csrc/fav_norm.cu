@@ -118,7 +118,7 @@ struct NormChannels {
     for (int i = 0; i < P; ++i) v[i] = f2fma(f2add(pair_of(x, i), make_float2(-mean, -mean)), w[i], b[i]);
     if (activation == FAV_ACTIVATION_SILU) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) v[i] = silu2(v[i]);
+      for (int i = 0; i < P; ++i) v[i] = silu2<T>(v[i]);
     } else if (activation == FAV_ACTIVATION_SNAKE) {
       float2 u[P], q[P];
       float far = 0.f;

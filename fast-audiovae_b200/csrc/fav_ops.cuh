@@ -143,18 +143,39 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
+// e^v, |v| <= 100. The argument of 2^x is off by the rounding of v log2 e, which
+// grows with v: in fp32 (T) what that lost is put back, e^v (1 + lost ln 2). Outputs of
+// 16 bits do without.
+constexpr float kLog2eLow = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
+template <typename T>
+__device__ __forceinline__ float exp_for(float v) {
+  const float t = v * kLog2e, e = ex2_approx(t);
+  if constexpr (sizeof(T) < 4) return e;
+  return e * fmaf(fmaf(v, kLog2eLow, fmaf(v, kLog2e, -t)), kLn2, 1.f);  // (infinity stays)
+}
+template <typename T>
+__device__ __forceinline__ float2 exp2_for(float2 v) {
+  const float2 t = f2mul(v, make_float2(kLog2e, kLog2e)), e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+  if constexpr (sizeof(T) < 4) return e;
+  const float2 lost = f2fma(v, make_float2(kLog2eLow, kLog2eLow),
+                            f2fma(v, make_float2(kLog2e, kLog2e), make_float2(-t.x, -t.y)));
+  return f2mul(e, f2fma(lost, make_float2(kLn2, kLn2), make_float2(1.f, 1.f)));
+}
+
 // v / (1 + e^-v) by the hardware's 2^x and 1/x (2 and 1 units in the last
 // place). Below -100, where e^-v overflows, v stands at -100: the result is
 // then 0, its limit, at -inf too. A NaN stays one.
+template <typename T>
 __device__ __forceinline__ float silu(float v) {
   v = max_nan(v, -100.f);
-  return v * rcp_approx(1.f + ex2_approx(-kLog2e * v));
+  return v * rcp_approx(1.f + exp_for<T>(sizeof(T) < 4 ? -v : -min_nan(v, 100.f)));
 }
 // The same of two, the multiplies and the sum packed.
+template <typename T>
 __device__ __forceinline__ float2 silu2(float2 v) {
   v = make_float2(max_nan(v.x, -100.f), max_nan(v.y, -100.f));
-  const float2 p = f2mul(v, make_float2(-kLog2e, -kLog2e));
-  const float2 s = f2add(make_float2(ex2_approx(p.x), ex2_approx(p.y)), make_float2(1.f, 1.f));
+  const float2 m = sizeof(T) < 4 ? make_float2(-v.x, -v.y) : make_float2(-min_nan(v.x, 100.f), -min_nan(v.y, 100.f));
+  const float2 s = f2add(exp2_for<T>(m), make_float2(1.f, 1.f));
   return f2mul(v, make_float2(rcp_approx(s.x), rcp_approx(s.y)));
 }
 

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float v = a.d ? fmaf(__ldg(a.d + c + i), to_f32(xv.v[i]), y[i]) : y[i];
-    if (a.z) v *= silu(to_f32(zv.v[i]));
+    if (a.z) v *= silu<T>(to_f32(zv.v[i]));
     out.v[i] = from_f32<T>(v);
   }
   store_pack<T, V>(static_cast<T*>(a.y) + s * a.y_stride + c, out);
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kBlockChannels* L, L == 2 ? 3 : 1) scan_kernel
         for (int k = 0; k < Q / L; ++k) {
           const int r = r0 + k * L + l;
           float v = fmaf(skip, to_f32(tile.x[r][ch]), y[k]);
-          if (gate) v *= silu(to_f32(tile.z[r][ch]));
+          if (gate) v *= silu<T>(to_f32(tile.z[r][ch]));
           tile.x[r][ch] = from_f32<T>(v);  // read by this lane alone
         }
       }

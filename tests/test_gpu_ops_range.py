@@ -335,3 +335,29 @@ def test_calls_see_what_their_own_stream_wrote(native, monkeypatch):
     for one, other in zip(want, got):
         for t, u in zip(one, other):
             assert torch.equal(t, u)
+
+
+def test_silu_in_fp32_keeps_its_digits():
+    """The same few roundings for any argument, by every operator that has it.
+
+    2^x errs by 2 units in the last place (4 U), the factor that corrects its argument and the product with it
+    by one rounding each, the sum by one, 1/x by a unit (2 U) and the product by one: 10 U. Below -87 the hardware
+    takes e^-v for infinity or its inverse, under 2^-126, for zero: 100 * 2^-126 is below 2e-36.
+    """
+    v = torch.cat([torch.linspace(-120, 120, 20_000), torch.linspace(-1, 1, 476),
+                   torch.tensor([-float("inf"), -3e38, -1e5, 3e38])]).view(1, -1)
+    wide = v.to(ref.WIDE).clamp(min=-500)   # the limit is zero
+    want = wide * torch.sigmoid(wide)
+    tol = 10 * ref.U * want.abs() * (1 + 1e-6) + 2e-36
+    n = v.shape[1]
+    one, d = torch.ones(1, n, device="cuda"), v.cuda()
+    close(ops.causal_conv(d, torch.tensor([[0.0, 1.0]], device="cuda").expand(n, 2).contiguous(), activation="silu"),
+          want, tol)
+    close(ops.causal_conv(d[None].expand(1, 1, n).repeat(1, 3, 1), torch.tensor([[0.0, 1.0]], device="cuda").expand(n, 2)
+                          .contiguous(), activation="silu")[0, :1], want, tol)   # behind it 0 * inf is no number
+    close(ops.group_norm(one, n // 8, None, d[0], activation="silu"), want, tol)
+    close(ops.group_norm(one.repeat(1, 3, 1), n // 8, None, d[0], activation="silu")[0, 1:2], want, tol)
+    none = torch.zeros(3, 1, 4, device="cuda")
+    close(ops.selective_scan(one, one, -torch.ones(4, n, device="cuda"), none[:1], none[:1], d=one[0], z=d), want, tol)
+    close(ops.selective_scan(*(one.repeat(1, 3, 1),) * 2, -torch.ones(4, n, device="cuda"), none[None], none[None], d=one[0],
+                             z=d.repeat(1, 3, 1))[0, 1:2], want, tol)
