@@ -45,15 +45,32 @@ View view(const void* p, long long stride, long long width, long long rows, int 
   return {static_cast<const char*>(p), stride * elem, width * elem, rows};
 }
 
+// Consecutive elements.
+View flat(const void* p, long long count, int elem) { return view(p, count, count, 1, elem); }
+
 // Whether two views share a byte. Views of one row stride may interleave (two
-// column ranges of one buffer); any other crossing counts as an overlap.
+// column ranges of one buffer), and a single row with the rows of a view; any other
+// crossing counts as an overlap.
 bool overlap(const View& a, const View& b) {
   if (!a.p || !b.p || a.rows == 0 || b.rows == 0) return false;
   const char *a_end = a.p + (a.rows - 1) * a.stride + a.width, *b_end = b.p + (b.rows - 1) * b.stride + b.width;
   if (a_end <= b.p || b_end <= a.p) return false;
-  if (a.stride != b.stride || a.stride <= 0 || a.rows == 1) return true;
-  const long long at = ((b.p - a.p) % a.stride + a.stride) % a.stride;
-  return at < a.width || at + b.width > a.stride;
+  if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+  const long long stride = a.rows > 1 ? a.stride : b.stride;
+  if ((a.rows == 1 && b.rows == 1) || stride <= 0) return true;
+  const long long at = ((b.p - a.p) % stride + stride) % stride;
+  return at < a.width || at + b.width > stride;
+}
+
+// Every array that a call writes is apart from the others and from what it reads.
+int32_t check_apart(std::initializer_list<View> written, std::initializer_list<View> read) {
+  for (const View* w = written.begin(); w != written.end(); ++w) {
+    for (const View& r : read)
+      if (overlap(*w, r)) return fail(FAV_OVERLAP, "outputs, state pool and workspace must not overlap the inputs");
+    for (const View* v = written.begin(); v != w; ++v)
+      if (overlap(*w, *v)) return fail(FAV_OVERLAP, "outputs, state pool and workspace must not overlap");
+  }
+  return FAV_OK;
 }
 
 int32_t check_stride(const char* name, int64_t stride, int32_t width, int32_t rows) {
@@ -116,10 +133,11 @@ int32_t fav_causal_conv(const fav_conv_args* args, void* cuda_stream) {
       (st = check_aligned(4, {c.weight, c.bias, c.slot_codes, c.offsets, c.status})) != FAV_OK)
     return st;
   const long long state = 2LL * (c.taps - 1) * c.channels;
-  const View x = view(c.x, c.x_stride, c.channels, c.rows, e), y = view(c.y, c.y_stride, c.channels, c.rows, e);
-  const View pool = view(c.state_pool, state, state, c.num_slots, e);
-  if (overlap(x, y) || overlap(x, pool) || overlap(y, pool))
-    return fail(FAV_OVERLAP, "x, y and the state pool must not overlap");
+  st = check_apart({view(c.y, c.y_stride, c.channels, c.rows, e), view(c.state_pool, state, state, c.num_slots, e),
+                    flat(c.status, 1, 4)},
+                   {view(c.x, c.x_stride, c.channels, c.rows, e), flat(c.weight, (long long)c.channels * c.taps, 4),
+                    flat(c.bias, c.channels, 4), flat(c.slot_codes, c.n, 4), flat(c.offsets, c.n + 1LL, 4)});
+  if (st != FAV_OK) return st;
   return launched(launch_causal_conv(c, sequences(c.offsets, c.slot_codes, c.n, c.length, c.rows, c.num_slots, c.status),
                                      static_cast<cudaStream_t>(cuda_stream)),
                   "convolution");
@@ -158,15 +176,16 @@ int32_t fav_selective_scan(const fav_scan_args* args, void* cuda_stream) {
       (st = check_aligned(4, {c.a, c.d, c.dt_bias, c.state_pool, c.slot_codes, c.offsets, c.status, c.workspace})) != FAV_OK)
     return st;
   const long long state = 2LL * c.states * c.channels;
-  const View y = view(c.y, c.y_stride, c.channels, c.rows, e);
-  const View pool = view(c.state_pool, state, state, c.num_slots, 4);
-  const View in[] = {view(c.x, c.x_stride, c.channels, c.rows, e), view(c.dt, c.dt_stride, c.channels, c.rows, e),
-                     view(c.z, c.z_stride, c.channels, c.rows, e),
-                     view(c.b, c.b_stride, (c.groups - 1) * (c.groups > 1 ? c.b_group_stride : 0) + c.states, c.rows, e),
-                     view(c.c, c.c_stride, (c.groups - 1) * (c.groups > 1 ? c.c_group_stride : 0) + c.states, c.rows, e)};
-  for (const View& v : in)
-    if (overlap(v, y) || overlap(v, pool)) return fail(FAV_OVERLAP, "y and the state pool must not overlap the inputs");
-  if (overlap(y, pool)) return fail(FAV_OVERLAP, "y must not overlap the state pool");
+  const long long b_width = (c.groups - 1) * (c.groups > 1 ? c.b_group_stride : 0) + c.states;
+  const long long c_width = (c.groups - 1) * (c.groups > 1 ? c.c_group_stride : 0) + c.states;
+  st = check_apart({view(c.y, c.y_stride, c.channels, c.rows, e), view(c.state_pool, state, state, c.num_slots, 4),
+                    flat(need ? c.workspace : nullptr, (long long)need, 1), flat(c.status, 1, 4)},
+                   {view(c.x, c.x_stride, c.channels, c.rows, e), view(c.dt, c.dt_stride, c.channels, c.rows, e),
+                    view(c.z, c.z_stride, c.channels, c.rows, e), view(c.b, c.b_stride, b_width, c.rows, e),
+                    view(c.c, c.c_stride, c_width, c.rows, e), flat(c.a, (long long)c.states * c.channels, 4),
+                    flat(c.d, c.channels, 4), flat(c.dt_bias, c.channels, 4), flat(c.slot_codes, c.n, 4),
+                    flat(c.offsets, c.n + 1LL, 4)});
+  if (st != FAV_OK) return st;
   return launched(launch_selective_scan(c, q, static_cast<cudaStream_t>(cuda_stream)), "scan");
 }
 
@@ -190,8 +209,10 @@ int32_t fav_group_norm(const fav_norm_args* args, void* cuda_stream) {
   if ((st = check_aligned(e, {c.x, c.y})) != FAV_OK ||
       (st = check_aligned(4, {c.weight, c.bias, c.alpha, c.reciprocal, c.offsets, c.status})) != FAV_OK)
     return st;
-  if (overlap(view(c.x, c.x_stride, c.channels, c.rows, e), view(c.y, c.y_stride, c.channels, c.rows, e)))
-    return fail(FAV_OVERLAP, "x and y must not overlap");
+  st = check_apart({view(c.y, c.y_stride, c.channels, c.rows, e), flat(c.status, 1, 4)},
+                   {view(c.x, c.x_stride, c.channels, c.rows, e), flat(c.weight, c.channels, 4), flat(c.bias, c.channels, 4),
+                    flat(c.alpha, c.channels, 4), flat(c.reciprocal, c.channels, 4), flat(c.offsets, c.n + 1LL, 4)});
+  if (st != FAV_OK) return st;
   return launched(launch_group_norm(c, sequences(c.offsets, nullptr, c.n, c.length, c.rows, 0, c.status),
                                     static_cast<cudaStream_t>(cuda_stream)),
                   "group norm");
@@ -213,8 +234,11 @@ int32_t fav_project_int4(const fav_int4_args* args, void* cuda_stream) {
   if (reinterpret_cast<uintptr_t>(c.weight) % 16) return fail(FAV_INVALID_ARGUMENT, "weight must be 16-byte aligned");
   const int e = elem_bytes(c.type);
   if ((st = check_aligned(e, {c.x, c.y})) != FAV_OK || (st = check_aligned(4, {c.scales, c.bias})) != FAV_OK) return st;
-  if (overlap(view(c.x, c.x_stride, c.depth, c.rows, e), view(c.y, c.y_stride, c.out, c.rows, e)))
-    return fail(FAV_OVERLAP, "x and y must not overlap");
+  const long long groups = ((long long)c.depth + c.group - 1) / c.group;
+  st = check_apart({view(c.y, c.y_stride, c.out, c.rows, e)},
+                   {view(c.x, c.x_stride, c.depth, c.rows, e), flat(c.weight, (long long)c.out * c.depth / 2, 1),
+                    flat(c.scales, c.out * groups, 4), flat(c.bias, c.out, 4)});
+  if (st != FAV_OK) return st;
   return launched(launch_project_int4(c, static_cast<cudaStream_t>(cuda_stream)), "projection");
 }
 

@@ -361,3 +361,17 @@ def test_silu_in_fp32_keeps_its_digits():
     close(ops.selective_scan(one, one, -torch.ones(4, n, device="cuda"), none[:1], none[:1], d=one[0], z=d), want, tol)
     close(ops.selective_scan(*(one.repeat(1, 3, 1),) * 2, -torch.ones(4, n, device="cuda"), none[None], none[None], d=one[0],
                              z=d.repeat(1, 3, 1))[0, 1:2], want, tol)
+
+
+def test_outputs_may_lie_between_other_rows():
+    """Coefficients in the columns that a strided output leaves free, and in a single row of them."""
+    buffer = torch.zeros(8, 256, device="cuda")
+    x = torch.randn(8, 64, device="cuda")
+    bias = buffer[3, 64:128]
+    bias.normal_()
+    assert torch.equal(ops.group_norm(x, 4, None, bias, out=buffer[:, :64]), ops.group_norm(x, 4, None, bias.clone()))
+    assert torch.equal(ops.group_norm(x, 4, None, bias, out=buffer[:, 192:]), ops.group_norm(x, 4, None, bias.clone()))
+    row = buffer[4:5, 64:128]
+    assert torch.equal(ops.group_norm(row, 4, out=buffer[4:5, 128:192]), ops.group_norm(row.clone(), 4))
+    with pytest.raises(_native.NativeError):
+        ops.group_norm(x, 4, None, bias, out=buffer[:, 64:128])

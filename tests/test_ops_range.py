@@ -172,3 +172,23 @@ def test_codes_into_a_given_tensor():
     for bad in (torch.zeros(3, dtype=torch.int32), torch.zeros(2), torch.zeros(4, dtype=torch.int32)[::2], [0, 0]):
         with pytest.raises(ValueError, match="out must be"):
             slots.codes([3, 1], out=bad)
+
+
+@pytest.mark.parametrize("name", list(ARRAYS))
+def test_outputs_over_any_input_are_refused(name):
+    """Each array that a call writes, at the address of each other one."""
+    lib = _native.load_library()
+    struct, sizes = SIZES[name]
+    if name == "fav_selective_scan":   # long enough for a workspace
+        sizes = dict(sizes, rows=2000)
+        sizes["workspace_bytes"] = lib.fav_selective_scan_workspace_bytes(ct.byref(struct(offsets=FAR, **sizes)))
+        assert sizes["workspace_bytes"]
+    arrays = {field: FAR * (i + 1) for i, field in enumerate(" ".join(ARRAYS[name]).split())}
+    if name == "fav_project_int4":
+        arrays["weight"] = sizes["weight"]
+        sizes = {k: v for k, v in sizes.items() if k != "weight"}
+    for written in ("y", "state_pool", "workspace", "status"):
+        for other in arrays:
+            if written in arrays and other != written:
+                args = struct(**sizes, **{**arrays, written: arrays[other]})
+                assert getattr(lib, name)(ct.byref(args), None) == 3, (written, other)
