@@ -482,6 +482,7 @@ def quantize_int4(weight, group):
     """
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError("weight must be a floating point tensor of shape [out, depth]")
+    weight = weight.detach()
     width, depth = weight.shape
     if type(group) is not int or group < 32 or group % 32 or depth < 32 or depth % 32:
         raise ValueError("group and the depth must be positive multiples of 32")

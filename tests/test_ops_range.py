@@ -192,3 +192,11 @@ def test_outputs_over_any_input_are_refused(name):
             if written in arrays and other != written:
                 args = struct(**sizes, **{**arrays, written: arrays[other]})
                 assert getattr(lib, name)(ct.byref(args), None) == 3, (written, other)
+
+
+def test_quantising_a_parameter_leaves_its_gradients_behind():
+    """Scales that wanted gradients would be refused by every projection."""
+    weight = torch.nn.Linear(64, 8).weight
+    packed, scales = ops.quantize_int4(weight, 32)
+    assert not scales.requires_grad and weight.requires_grad
+    assert all(torch.equal(*pair) for pair in zip((packed, scales), ops.quantize_int4(weight.detach(), 32)))
