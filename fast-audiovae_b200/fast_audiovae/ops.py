@@ -521,8 +521,8 @@ class StreamSlots:
     """
 
     def __init__(self, slots, *, device="cuda"):
-        if type(slots) is not int or slots < 1:
-            raise ValueError("slots must be a positive int")
+        if type(slots) is not int or not 1 <= slots <= _SLOTS:
+            raise ValueError("slots must be a positive int, up to 2^29")
         self.device = torch.device(device)
         self._table = np.zeros(slots, np.int32)
         self._fresh = np.ones(slots, np.int32)

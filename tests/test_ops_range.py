@@ -200,3 +200,10 @@ def test_quantising_a_parameter_leaves_its_gradients_behind():
     packed, scales = ops.quantize_int4(weight, 32)
     assert not scales.requires_grad and weight.requires_grad
     assert all(torch.equal(*pair) for pair in zip((packed, scales), ops.quantize_int4(weight.detach(), 32)))
+
+
+@pytest.mark.parametrize("slots", [0, 2 ** 29 + 1, 2 ** 31, 4.0])
+def test_slots_that_codes_cannot_name_are_refused(slots):
+    """A code holds a slot's number in 29 bits."""
+    with pytest.raises(ValueError, match="slots must be"):
+        ops.StreamSlots(slots, device="cpu")
