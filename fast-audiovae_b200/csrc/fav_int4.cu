@@ -3,10 +3,10 @@
 //   y[m, r] = bias[r] + sum_g scales[r, g] * sum_{k in g} x[m, k] * (q[r, k] - 8)
 //
 // The floor is reading the weights once (out * depth / 2 bytes: 2.8 us of 16 x
-// 8192 x 4096, 0.7 us of 1 x 4096 x 2048). They take 10.9 and 4.2 us: the chain of
-// launch, weights, inputs, products and join, a few us long, and for more input
-// rows the reading and arranging of inputs from L1. The codes minus 8 are exact
-// in fp16 and bf16, so the inner sums run on the tensor cores with
+// 8192 x 4096, 0.7 us of 1 x 4096 x 2048). They take 12.4 and 4.8 us, with weights that
+// are in L2 already 10.6 and 3.9: the chain of launch, weights, inputs, products and
+// join, a few us long, and for more input rows the reading and arranging of inputs
+// from L1. The codes minus 8 are exact in fp16 and bf16, so the inner sums run on the tensor cores with
 // exact operands: mma.sync m16n8k16, 16 weight rows by 8 input rows, fp32
 // accumulation (an input row or two cannot fill a tcgen05 tile, and the codes
 // must pass the registers anyway to become operands). A block's sum is scaled
@@ -22,7 +22,7 @@
 // join through shared memory in a fixed order. Many warps with short loops hide
 // more than few with long ones: a warp has U blocks of weights and inputs on
 // their way at once, 16 bytes of weights a lane and row. (Twice and four times as
-// much, 1 x 64 x 4096 3.8 and 4.9 us instead of 3.4: straight code that runs once
+// much, 1 x 4096 x 2048 7.2 and 9.2 us instead of 4.8: straight code that runs once
 // costs more to fetch than the wait it saves.)
 // Sums of inputs times codes may leave fp32's range where the scaled ones do not
 // (bf16 and fp32 inputs above 2^117; fp16 stays far below). A thread that finds
@@ -317,8 +317,8 @@ template <typename T, bool WIDE, int W>
 cudaError_t launch_width(const Int4Args& a, cudaStream_t stream) {
   // Up to 32 input rows share a pass over the weights. More weight rows a CTA
   // where that still gives every SM one: the inputs are then read and arranged
-  // less often (16 inputs of 8192 x 4096: 16 rows 16 us, 32 rows 12.5, 64 rows in
-  // the registers of eight warps 10.9).
+  // less often (16 inputs of 8192 x 4096: 16 rows 16.5 us, 32 rows 14.5, 64 rows in
+  // the registers of eight warps 12.4).
   const bool many = a.out >= 148 * 32;
   if (a.rows <= 8) return many ? launch_tile<T, WIDE, W, 2, 1, 16>(a, stream) : launch_tile<T, WIDE, W, 1, 1, 16>(a, stream);
   if (a.rows <= 16) return many ? launch_tile<T, WIDE, W, 4, 2, 8>(a, stream) : launch_tile<T, WIDE, W, 2, 2, 16>(a, stream);

@@ -6,10 +6,10 @@
 // squares. A running sum of values far from zero is off by its own roundings
 // (a clip of 6000 x 2048 values 1000.1 in one group: its mean by 0.004), so the pass
 // that sums the squares of x - mean sums those differences too: their mean corrects
-// both. A mean is kept as two floats, the second one part of the bias, and threads
-// and blocks join by (count, mean, sum of squares about it) with means as offsets
-// from one of them: a mean far from zero costs no digits but its square's in U.
-// The order of every sum is fixed.
+// both (64 clips of 750 x 512: 1 % more time in fp32, 5 % in 16 bits). A mean is kept as
+// two floats, the second one part of the bias, and threads and blocks join by (count,
+// mean, sum of squares about it) with means as offsets from one of them: of a mean far
+// from zero a second-order rounding is left. The order of every sum is fixed.
 //
 // Bound by memory: x is read once and y written once. Single rows keep a group
 // in the registers of 1 to 256 threads. Longer sequences are cut into blocks of
@@ -17,7 +17,7 @@
 // CTAs shares a block's rows: each keeps its rows in shared memory, the CTAs
 // exchange their statistics through distributed shared memory, and y is formed
 // from the kept rows. Rows beyond the shared memory are read again (from L2
-// mostly). 64 clips of 750 x 512 fp32 take 43 us, 70 % of the copy rate: a CTA
+// mostly). 64 clips of 750 x 512 fp32 take 43 us, 69 % of the copy rate: a CTA
 // loads, exchanges and stores in turn, so that only several an SM overlap. (Two
 // launches over ranges of rows, which read x twice, took 57 us, and two to four
 // times as long where sequences are short.)
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kRowThreads) norm_rows_kernel(const __grid_con
 
 constexpr int kWideThreads = 512;  // of a CTA with a large share of the rows
 // Of a CTA with a small one: twice as many for fp32 (64 clips of 750 x 512: 256
-// threads 43 us, 128 45 us; bf16 34 and 30).
+// threads 43 us, 128 48 us; bf16 with SiLU 44 and 35).
 constexpr int small_threads(int v) { return v == 4 ? 256 : 128; }
 constexpr int kMaxCtas = 16;  // of a cluster (above 8 where the device can place them)
 
@@ -339,8 +339,9 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
     const long long hop = dr * a.x_stride;
     if constexpr (V == 8) {
       // 16 vectors are on their way to their places, four of them summed at a
-      // time: the sums of 8 take long enough to hide loads behind (64 clips of
-      // 750 x 512 bf16: 29 us, all rows first 36).
+      // time, so that the sums of 8 hide loads (bf16 with SiLU, all rows first in
+      // brackets: 4 clips of 150 x 512 6.7 us (7.7), 64 of 1500 93 (95), 64 of 750
+      // 34.7 both, 64 of 12 9.7 (9.2)).
       int issued = 0;
       const auto issue = [&] {
 #pragma unroll
@@ -359,8 +360,8 @@ __global__ void __launch_bounds__(NT, NT == kWideThreads ? 1 : 4) norm_kernel(co
           if (k + u < kept_vectors) sums = add_values(to[(k + u) * step], sums);
       }
     } else {
-      // All of the kept rows are on their way at once, then summed (fp32 44 us, as
-      // above 49).
+      // All of the kept rows are on their way at once, then summed (64 clips of 750 x
+      // 512 fp32 43 us, as above 45).
 #pragma unroll 4
       for (int k = 0; k < kept_vectors; ++k, p += hop) copy_pack<T, V>(to + k * step, p);
       copy_commit();

@@ -143,10 +143,11 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
-// e^v, |v| <= 100. The argument of 2^x is off by the rounding of v log2 e, which
-// grows with v: in fp32 (T) what that lost is put back, e^v (1 + lost ln 2). Outputs of
-// 16 bits do without.
-constexpr float kLog2eLow = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
+// e^v, |v| <= 100, and of two. The argument of 2^x is off by the rounding of v log2 e,
+// which grows with v (25 units of e^v at 20): in fp32 (T) what that and the rounding of
+// log2 e itself lost is put back, e^v (1 + lost ln 2). Outputs of 16 bits do without.
+constexpr float kLog2eLow = 1.9259629911266175e-8f;  // log2 e less the float
+constexpr float kLn2 = 0.6931471805599453f;
 template <typename T>
 __device__ __forceinline__ float exp_for(float v) {
   const float t = v * kLog2e, e = ex2_approx(t);
@@ -154,7 +155,7 @@ __device__ __forceinline__ float exp_for(float v) {
   return e * fmaf(fmaf(v, kLog2eLow, fmaf(v, kLog2e, -t)), kLn2, 1.f);  // (infinity stays)
 }
 template <typename T>
-__device__ __forceinline__ float2 exp2_for(float2 v) {
+__device__ __forceinline__ float2 exp_pair(float2 v) {
   const float2 t = f2mul(v, make_float2(kLog2e, kLog2e)), e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
   if constexpr (sizeof(T) < 4) return e;
   const float2 lost = f2fma(v, make_float2(kLog2eLow, kLog2eLow),
@@ -175,7 +176,7 @@ template <typename T>
 __device__ __forceinline__ float2 silu2(float2 v) {
   v = make_float2(max_nan(v.x, -100.f), max_nan(v.y, -100.f));
   const float2 m = sizeof(T) < 4 ? make_float2(-v.x, -v.y) : make_float2(-min_nan(v.x, 100.f), -min_nan(v.y, 100.f));
-  const float2 s = f2add(exp2_for<T>(m), make_float2(1.f, 1.f));
+  const float2 s = f2add(exp_pair<T>(m), make_float2(1.f, 1.f));
   return f2mul(v, make_float2(rcp_approx(s.x), rcp_approx(s.y)));
 }
 

@@ -64,8 +64,8 @@ __device__ __forceinline__ float times_power(float h, float p) {
 // bytes a channel), so a thread moves V = 4 neighbouring channels of a state
 // with 16-byte accesses; L lanes of a warp share a channel's states where
 // there are too few channels and streams to fill the GPU. 512 streams of 2048 x 16
-// take 27.5 us, 70 % of the copy rate; without the hint that a state is not used
-// again 31. (Holding `a` in registers over several streams took 51 us: the
+// take 27 us, 71 % of the copy rate; without the hint that a state is not used
+// again 30. (Holding `a` in registers over several streams took 51 us: the
 // registers cost more warps than the reads of `a` time.)
 constexpr int kStepThreads = 128;
 
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
     y[i] = 0.f;
   }
   const bool held = st.slot >= 0 && st.read >= 0, keep = live && st.slot >= 0;
-  constexpr int B = 4;  // states of a lane on their way at once (eight: fewer warps, 36 us)
+  constexpr int B = 4;  // states of a lane on their way at once (four: 26.7 us, eight, with fewer warps: 27.3)
   for (int n0 = l; n0 < a.states; n0 += B * L) {
     Pack<float, V> h[B];
 #pragma unroll
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(const __grid_co
 //
 // Bound by the special function unit: T * C * N times ex2 at 16 a clock and SM,
 // and four more a value for softplus and gate. 32 ragged prompts of up to 750 x
-// 1536 x 16 in fp32 need 100 us of it and take 167: it is busy two thirds of the
+// 1536 x 16 in fp32 need 100 us of it and take 168: it is busy two thirds of the
 // time on the SMs that have work, and the SMs' shares differ. (A quarter of the
 // powers by a polynomial on the FMA pipe took 10 % longer: the instructions it
 // adds are as scarce.)
@@ -450,7 +450,7 @@ template <typename T, int V>
 cudaError_t launch_step(const ScanArgs& a, cudaStream_t stream) {
   const long long items = (long long)a.seq.n * (a.channels / V);
   // Four lanes per channel vector while one would leave an SM under 1024 threads,
-  // sixteen while four would leave it under 128 (1 x 1024 channels 2.6 us, not 3.1).
+  // sixteen while four would leave it under 128 (1 x 1024 channels 2.4 us, not 2.9).
   const int lanes = items >= 148 * 1024 ? 1 : items >= 148 * 32 ? 4 : 16;
   const long long blocks = (items * lanes + kStepThreads - 1) / kStepThreads;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;

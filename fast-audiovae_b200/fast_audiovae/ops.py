@@ -33,8 +33,9 @@ the arrays is touched.
 Coefficients are contiguous fp32; sums, states and statistics run in fp32, and
 every output is rounded once to its type. Work is enqueued on the current
 stream of the tensors' device without synchronising and may be captured in a
-CUDA graph. The operators are for inference and have no gradients. They run in
-``libfav_cuda.so``; there is no CPU path.
+CUDA graph. The operators are for inference: tensors that want gradients or
+carry forward derivatives are refused, states and outputs among them. They run
+in ``libfav_cuda.so``; there is no CPU path.
 """
 from __future__ import annotations
 
