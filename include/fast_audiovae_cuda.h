@@ -313,7 +313,8 @@ FAV_API int32_t fav_causal_conv(const fav_conv_args *args, void *cuda_stream);
  * strides; a: [N][channels]. state_pool: [num_slots][2][N][channels] fp32.
  * z, d and dt_bias may be NULL. Long sequences that are too few to fill the
  * GPU are cut into pieces, whose states need `workspace`
- * (fav_selective_scan_workspace_bytes, which reads sizes only; 0 for a step). */
+ * (fav_selective_scan_workspace_bytes, which reads sizes and whether offsets is
+ * NULL; 0 for a step). */
 typedef struct fav_scan_args {
   const void *x, *dt, *z, *b, *c;
   void *y;

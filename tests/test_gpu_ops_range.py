@@ -375,3 +375,35 @@ def test_outputs_may_lie_between_other_rows():
     assert torch.equal(ops.group_norm(row, 4, out=buffer[4:5, 128:192]), ops.group_norm(row.clone(), 4))
     with pytest.raises(_native.NativeError):
         ops.group_norm(x, 4, None, bias, out=buffer[:, 64:128])
+
+
+def test_two_threads_call_at_once():
+    """Calls give the interpreter's lock back while they launch; each thread's stream and tensors are its own."""
+    g = gen(60)
+    w, a = torch.randn(64, 4, generator=g).cuda(), -torch.rand(4, 64, generator=g).cuda()
+    weight, scales = torch.randint(0, 256, (40, 32), generator=g, dtype=torch.uint8).cuda(), torch.ones(40, 2, device="cuda")
+
+    def run(x):
+        maps = x[:, :4].unsqueeze(1)
+        return [ops.causal_conv(x, w), ops.group_norm(x[None], 8), ops.selective_scan(x[None], x[None], a, maps[None], maps[None]),
+                ops.project_int4(x, weight, scales, group=32)]
+
+    data = torch.randn(2, 300, 64, generator=g).cuda()
+    want = [run(x) for x in data]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(100):
+                got = run(data[i])
+                if not all(torch.equal(t, u) for t, u in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
